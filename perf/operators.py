@@ -254,7 +254,7 @@ def _prepare_attention(s, c, gen, dtype):
                               max_k=max(n for _, n in s.k_at), q_starts=s.q_starts.data_ptr(), k_starts=s.k_starts.data_ptr(),
                               k_lens=s.k_lens.data_ptr(), causal=int(c["causal"]), scale=s.scale)
         if c["direction"] == "step":
-            s.delta = torch.empty((hq, rows_q), device="cuda", dtype=torch.float32)
+            s.scratch = torch.empty(s.plan.bw_scratch_floats(), device="cuda", dtype=torch.float32)
             if c["fused"]:  # the gradients go where the product's backward pass wants them
                 gqkv = torch.empty((rows_q, hq + 2 * hk, d), device="cuda", dtype=dtype)
                 s.gq, s.gk, s.gv = gqkv[:, :hq], gqkv[:, hq:hq + hk], gqkv[:, hq + hk:]
@@ -304,7 +304,7 @@ def _attention_own(s):
         return s.y
     s.ctx.attention_fw(s.mode, s.plan, s.q.data_ptr(), s.k.data_ptr(), s.v.data_ptr(), s.y.data_ptr(), s.lse.data_ptr(), stream=at)
     s.ctx.attention_bw(s.mode, s.plan, s.q.data_ptr(), s.k.data_ptr(), s.v.data_ptr(), s.y.data_ptr(), s.lse.data_ptr(), s.gy.data_ptr(),
-                       s.gq.data_ptr(), s.gk.data_ptr(), s.gv.data_ptr(), s.delta.data_ptr(), accumulate=False, stream=at)
+                       s.gq.data_ptr(), s.gk.data_ptr(), s.gv.data_ptr(), s.scratch.data_ptr(), accumulate=False, stream=at)
     return s.y, s.gq, s.gk, s.gv
 
 
