@@ -9,4 +9,5 @@ library is missing, or no sm_100 GPU is visible, the calls raise.
 """
 from .capi import (  # noqa: F401
     MODE_FP32_3XTF32, MODE_TF32, MODE_FP16, MODE_FP32_3XFP16, B200Error, Context, lib, library_path,
+    Attention, NORM_ROTARY_SCRATCH, ROTARY_HALVES, ROTARY_PAIRS, rotary_frequencies,
 )

@@ -18,6 +18,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "../../include/primitiv_b200_attention.h"
 #include "../../include/primitiv_b200_ops.h"
 
 namespace {
@@ -96,7 +97,8 @@ const Named kEntries[] = {
     B200_ENTRY(b200_pick_bw), B200_ENTRY(b200_broadcast_fw), B200_ENTRY(b200_batch_pick_fw),
     B200_ENTRY(b200_batch_pick_bw), B200_ENTRY(b200_transpose), B200_ENTRY(b200_permute_dims), B200_ENTRY(b200_flip),
     B200_ENTRY(b200_reduce_fw), B200_ENTRY(b200_minmax_bw), B200_ENTRY(b200_argminmax), B200_ENTRY(b200_batch_sum_fw),
-    B200_ENTRY(b200_random),
+    B200_ENTRY(b200_random), B200_ENTRY(b200_rotary_fw), B200_ENTRY(b200_rotary_bw), B200_ENTRY(b200_norm_rotary_fw),
+    B200_ENTRY(b200_norm_rotary_bw), B200_ENTRY(b200_attention_fw), B200_ENTRY(b200_attention_bw),
 };
 #undef B200_ENTRY
 

@@ -18,6 +18,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(CSRC, "_obj")
 LIB = os.path.join(PKG, "libprimitiv_b200.so")
+HEADERS = ("primitiv_b200.h", "primitiv_b200_ops.h", "primitiv_b200_attention.h")
 BINDING = os.path.join(PKG, "binding", "native.cc")
 # CPython module over the library.  The name carries the interpreter's tag, so that another interpreter does not import it.
 NATIVE = os.path.join(PKG, "_native" + sysconfig.get_config_var("EXT_SUFFIX"))
@@ -54,7 +55,7 @@ def _build_native(force):
     if not os.path.exists(os.path.join(include, "Python.h")):
         sys.stderr.write("note: no Python.h in %s; calls go through ctypes (5.3 us instead of 2.7)\n" % include)
         return
-    headers = [os.path.join(os.path.dirname(PKG), "include", f) for f in ("primitiv_b200.h", "primitiv_b200_ops.h")]
+    headers = [os.path.join(os.path.dirname(PKG), "include", f) for f in HEADERS]
     if not force and not _stale(NATIVE, [BINDING, os.path.abspath(__file__)] + headers):
         return
     cmd = ["g++", "-O3", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", "-I" + include, BINDING, "-o", NATIVE,
@@ -78,8 +79,7 @@ def build(verbose=False, force=False, dev_knobs=False):
     if old_flags != " ".join(flags):
         force = True
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
-    headers.append(os.path.join(os.path.dirname(PKG), "include", "primitiv_b200.h"))
-    headers.append(os.path.join(os.path.dirname(PKG), "include", "primitiv_b200_ops.h"))
+    headers += [os.path.join(os.path.dirname(PKG), "include", f) for f in HEADERS]
     headers.append(os.path.abspath(__file__))
     jobs = []
     objs = []

@@ -103,7 +103,50 @@ SIGNATURES = {
     "b200_peer_enable": (_int, [_vp, _vp]),
     "b200_stream_barrier": (_int, [ctypes.POINTER(_vp), _int]),
     "b200_peer_sum": (_int, [_vp, _int, ctypes.POINTER(_vp), _int, _vp, _u64, _int, _vp]),
+    # ---- include/primitiv_b200_attention.h ----
+    "b200_rotary_frequencies": (_int, [_u32, ctypes.c_double, _int, ctypes.c_double, ctypes.c_double, _vp, _vp]),
+    "b200_rotary_fw": (_int, [_vp, _int, _vp, _vp, _u32, _u32, _u32, _u64, _u64, _u32, _int, _vp, ctypes.c_float, _vp, _vp]),
+    "b200_rotary_bw": (_int, [_vp, _int, _vp, _vp, _u32, _u32, _u32, _u64, _u64, _u32, _int, _vp, ctypes.c_float, _vp, _int, _vp]),
+    "b200_norm_rotary_fw": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u64, _u64, _u32, _int, _vp,
+                                   ctypes.c_float, _vp, ctypes.c_float, _vp]),
+    "b200_norm_rotary_bw": (_int, [_vp, _int] + [_vp] * 8 + [_u32] * 4 + [_u64] * 3 + [_u32, _int, _vp, ctypes.c_float, _vp,
+                                   ctypes.c_float, _int, _int, _vp]),
+    "b200_attention_fw": (_int, [_vp, _int] + [_vp] * 7),
+    "b200_attention_bw": (_int, [_vp, _int] + [_vp] * 11 + [_int, _vp]),
+    "b200_attention_bw_scratch": (_int, [_vp, _vp]),
 }
+
+ROTARY_PAIRS = 0
+ROTARY_HALVES = 1
+ROTARY_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "by_parts": 3}
+NORM_ROTARY_SCRATCH = 512 * 512   # floats
+
+
+class Attention(ctypes.Structure):
+    """The plan of an attention: sizes, strides and sequences (b200_attention, primitiv_b200_attention.h).
+    Fields that are not given are 0 or None; q_starts, q_lens, k_starts and k_lens are addresses of uint32 arrays
+    on the device, which the caller keeps alive."""
+    _fields_ = [("head", _u32), ("heads_q", _u32), ("heads_k", _u32), ("rows_q", _u32), ("rows_k", _u32),
+                ("seqs", _u32), ("max_q", _u32), ("max_k", _u32),
+                ("q_ld", _u64), ("k_ld", _u64), ("v_ld", _u64), ("y_ld", _u64),
+                ("q_starts", _vp), ("q_lens", _vp), ("k_starts", _vp), ("k_lens", _vp),
+                ("causal", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+    def bw_scratch_floats(self):
+        """Floats of scratch that attention_bw wants for this plan."""
+        n = _u64()
+        _check(lib().b200_attention_bw_scratch(ctypes.addressof(self), ctypes.addressof(n)), "attention_bw_scratch")
+        return n.value
+
+
+def rotary_frequencies(rot, base=10000.0, scaling="plain", factor=1.0, original=0.0):
+    """-> (list of rot/2 frequencies in radians per position, amplitude); scaling: "plain", "linear", "base", "by_parts"."""
+    freqs, amplitude = (ctypes.c_double * max(rot // 2, 1))(), ctypes.c_double()
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError("scaling: one of " + ", ".join(ROTARY_SCALINGS))
+    _check(lib().b200_rotary_frequencies(rot, base, ROTARY_SCALINGS[scaling], factor, original, ctypes.addressof(freqs),
+                                         ctypes.addressof(amplitude)), "rotary_frequencies")
+    return list(freqs[:rot // 2]), amplitude.value
 
 
 class B200Error(RuntimeError):
@@ -289,6 +332,35 @@ class Context:
 
     def selftest_wait_timeout(self, stream=None):
         _check(lib().b200_selftest_wait_timeout(self._h, stream), "selftest_wait_timeout")
+
+    # -- attention layers (primitiv_b200_attention.h; device pointers as ints) --
+    def rotary_fw(self, mode, x, y, head, heads, tokens, x_ld, y_ld, rot, layout, freqs, amplitude=1.0, positions=None,
+                  stream=None):
+        self.op("b200_rotary_fw", mode, x, y, head, heads, tokens, x_ld, y_ld, rot, layout, freqs, amplitude, positions, stream)
+
+    def rotary_bw(self, mode, gy, gx, head, heads, tokens, gy_ld, gx_ld, rot, layout, freqs, amplitude=1.0, positions=None,
+                  accumulate=True, stream=None):
+        self.op("b200_rotary_bw", mode, gy, gx, head, heads, tokens, gy_ld, gx_ld, rot, layout, freqs, amplitude, positions,
+                int(accumulate), stream)
+
+    def norm_rotary_fw(self, mode, x, gain_q, gain_k, y, head, heads_q, heads_k, tokens, x_ld, y_ld, rot, layout, freqs,
+                       amplitude=1.0, positions=None, eps=1e-6, stream=None):
+        self.op("b200_norm_rotary_fw", mode, x, gain_q, gain_k, y, head, heads_q, heads_k, tokens, x_ld, y_ld, rot, layout, freqs,
+                amplitude, positions, eps, stream)
+
+    def norm_rotary_bw(self, mode, x, gain_q, gain_k, gy, gx, ggain_q, ggain_k, scratch, head, heads_q, heads_k, tokens, x_ld,
+                       gy_ld, gx_ld, rot, layout, freqs, amplitude=1.0, positions=None, eps=1e-6, accumulate_x=True,
+                       accumulate_gain=True, stream=None):
+        """scratch: NORM_ROTARY_SCRATCH floats on the device (None where neither gain's gradient is wanted)."""
+        self.op("b200_norm_rotary_bw", mode, x, gain_q, gain_k, gy, gx, ggain_q, ggain_k, scratch, head, heads_q, heads_k, tokens,
+                x_ld, gy_ld, gx_ld, rot, layout, freqs, amplitude, positions, eps, int(accumulate_x), int(accumulate_gain), stream)
+
+    def attention_fw(self, mode, plan, q, k, v, y, lse=None, stream=None):
+        self.op("b200_attention_fw", mode, ctypes.addressof(plan), q, k, v, y, lse, stream)
+
+    def attention_bw(self, mode, plan, q, k, v, y, lse, gy, gq, gk, gv, scratch, accumulate=True, stream=None):
+        """scratch: plan.bw_scratch_floats() floats on the device."""
+        self.op("b200_attention_bw", mode, ctypes.addressof(plan), q, k, v, y, lse, gy, gq, gk, gv, scratch, int(accumulate), stream)
 
     def op(self, name, *args):
         """Calls any other entry point by name (the elementwise / movement / reduction set).  Where

@@ -1,0 +1,603 @@
+// Attention with mma.sync: every storage type, head size, stride and alignment.
+//
+// One block has 64 rows of one key head and walks the other side in tiles, everything between two products staying in
+// registers: the accumulator of s = q k^T has the layout that the next product wants of its left operand.  A row is a
+// query of one of the `group` heads that share a key head, so those read its keys once: row r of a sequence is query
+// r / group, head r % group.
+//
+// forward:  the running maximum m and sum l of a softmax; y = y 2^(m - m') + p v, one pass over the keys.
+// backward: p is computed again from lse.  Two kernels of the same shape, one with the keys at rest (gk, gv), one with
+//   the queries (gq): s and dp are computed twice, which costs 7 products instead of 5 and needs neither atomics nor
+//   a sum over blocks, so the same call has the same bits.
+//
+// fp32 storage: a product is three TF32 passes on x = hi + lo split in registers (one in B200_MODE_TF32).  The tensor core
+// truncates as it adds into its accumulator, so no sum runs longer than one tile there: each tile's product starts from zero and
+// is added in fp32 instructions.  Halves: p and ds are rounded to half for the second product, ds after a scale by a power of
+// two (see scale_of), without which the ds of a long row, p / row length times a small gy, would lie below the
+// smallest half.
+#include <algorithm>
+#include <type_traits>
+
+#include "attention.h"
+
+namespace b200 {
+namespace {
+
+constexpr uint32_t kRows = 64;       // rows at rest per block
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kPScale = 8192.f;    // backward, halves: p in [0, 1] times this
+
+__device__ __forceinline__ uint32_t smem_at(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// ---- fragments and products --------------------------------------------------------------------------------
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// x = hi + lo in TF32.  An infinity or a NaN stays in hi, with lo = 0: the difference would be a NaN.
+template <int kPass>
+__device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  if constexpr (kPass == 3) {
+    const float rest = x - __uint_as_float(hi);
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(fabsf(x) <= 3.0e38f ? rest : 0.f));
+  }
+}
+
+// Row pitch of a tile in shared memory, in elements: 16 bytes more than the row, so that eight rows start in eight different
+// groups of banks.
+template <typename T, int kD> constexpr int kPitch = kD + 16 / static_cast<int>(sizeof(T));
+
+// c[16 rows of this warp][8 NT] = X . Y^T, X and Y with contiguous rows of kD elements.
+template <int kD, int NT, int kPass>
+__device__ __forceinline__ void product_abt(float (&c)[NT][4], const __half *x, const __half *y) {
+  constexpr int P = kPitch<__half, kD>;
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint32_t xa = smem_at(x) + ((lane & 15u) * P + (lane >> 4) * 8u) * 2u;
+  const uint32_t ya = smem_at(y) + (((lane & 7u) + (lane >> 4) * 8u) * P + ((lane >> 3) & 1u) * 8u) * 2u;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < kD / 16; ++kk) {
+    uint32_t a[4], b[4];
+    ldsm4(a, xa + kk * 32);
+#pragma unroll
+    for (int n = 0; n < NT; n += 2) {
+      ldsm4(b, ya + (n * 8 * P + kk * 16) * 2);
+      mma_f16(c[n], a, b[0], b[1]);
+      mma_f16(c[n + 1], a, b[2], b[3]);
+    }
+  }
+}
+template <int kD, int NT, int kPass>
+__device__ __forceinline__ void product_abt(float (&c)[NT][4], const float *x, const float *y) {
+  constexpr int P = kPitch<float, kD>;
+  const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+  const float *xa = x + g * P + t, *ya = y + g * P + t;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
+#pragma unroll 4
+  for (int kk = 0; kk < kD / 8; ++kk) {
+    uint32_t ah[4], al[4];
+    split<kPass>(xa[kk * 8], ah[0], al[0]);
+    split<kPass>(xa[8 * P + kk * 8], ah[1], al[1]);
+    split<kPass>(xa[kk * 8 + 4], ah[2], al[2]);
+    split<kPass>(xa[8 * P + kk * 8 + 4], ah[3], al[3]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      uint32_t bh[2], bl[2];
+      split<kPass>(ya[n * 8 * P + kk * 8], bh[0], bl[0]);
+      split<kPass>(ya[n * 8 * P + kk * 8 + 4], bh[1], bl[1]);
+      if constexpr (kPass == 3) {
+        mma_tf32(c[n], al, bh[0], bh[1]);
+        mma_tf32(c[n], ah, bl[0], bl[1]);
+      }
+      mma_tf32(c[n], ah, bh[0], bh[1]);
+    }
+  }
+}
+
+// acc[16 rows][kCols columns from col0] = acc * keep[row half] + P . Y, P in the accumulator layout [NT tiles of 8], Y of 8 NT rows.
+template <int kD, int kCols, int NT, int kPass>
+__device__ __forceinline__ void product_py(float (&acc)[kCols / 8][4], const float (&p)[NT][4], const __half *y, int col0, float keep0, float keep1) {
+  constexpr int P = kPitch<__half, kD>;
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint32_t ya = smem_at(y) + ((lane & 15u) * P + (lane >> 4) * 8u + col0) * 2u;
+  uint32_t a[NT / 2][4];
+#pragma unroll
+  for (int j = 0; j < NT / 2; ++j) {
+    a[j][0] = half2_of(p[2 * j][0], p[2 * j][1]);
+    a[j][1] = half2_of(p[2 * j][2], p[2 * j][3]);
+    a[j][2] = half2_of(p[2 * j + 1][0], p[2 * j + 1][1]);
+    a[j][3] = half2_of(p[2 * j + 1][2], p[2 * j + 1][3]);
+  }
+#pragma unroll
+  for (int n = 0; n < kCols / 8; n += 2) {
+    float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NT / 2; ++j) {
+      uint32_t b[4];
+      ldsm4t(b, ya + (j * 16 * P + n * 8) * 2);
+      mma_f16(c0, a[j], b[0], b[1]);
+      mma_f16(c1, a[j], b[2], b[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float keep = i < 2 ? keep0 : keep1;
+      acc[n][i] = acc[n][i] * keep + c0[i];
+      acc[n + 1][i] = acc[n + 1][i] * keep + c1[i];
+    }
+  }
+}
+// The accumulator has columns 2t, 2t+1 where the left operand wants k = t, t+4: the rows of Y are taken in that order instead.
+template <int kD, int kCols, int NT, int kPass>
+__device__ __forceinline__ void product_py(float (&acc)[kCols / 8][4], const float (&p)[NT][4], const float *y, int col0, float keep0, float keep1) {
+  constexpr int P = kPitch<float, kD>;
+  const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+  const float *ya = y + 2 * t * P + g + col0;
+  uint32_t ah[NT][4], al[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    split<kPass>(p[j][0], ah[j][0], al[j][0]);
+    split<kPass>(p[j][2], ah[j][1], al[j][1]);
+    split<kPass>(p[j][1], ah[j][2], al[j][2]);
+    split<kPass>(p[j][3], ah[j][3], al[j][3]);
+  }
+#pragma unroll
+  for (int n = 0; n < kCols / 8; ++n) {
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      uint32_t bh[2], bl[2];
+      split<kPass>(ya[j * 8 * P + n * 8], bh[0], bl[0]);
+      split<kPass>(ya[j * 8 * P + P + n * 8], bh[1], bl[1]);
+      if constexpr (kPass == 3) {
+        mma_tf32(c, al[j], bh[0], bh[1]);
+        mma_tf32(c, ah[j], bl[0], bl[1]);
+      }
+      mma_tf32(c, ah[j], bh[0], bh[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = acc[n][i] * (i < 2 ? keep0 : keep1) + c[i];
+  }
+}
+
+// ---- tiles ---------------------------------------------------------------------------------------------
+
+// Rows [row0, row0 + ROWS) of a side into shared memory, zeros past `rows` and past `head`.  Row r is token r / per, head
+// r % per behind `base` (per = 1: plain rows).  Copied in 16-byte pieces where every address allows, and then still in
+// flight on return.
+template <typename T, int kD, int ROWS, int kThreads>
+__device__ __forceinline__ void load_rows(T *dst, const T *base, unsigned long long ld, uint32_t per, uint32_t row0, uint32_t rows, uint32_t head, bool wide) {
+  constexpr int P = kPitch<T, kD>, N = 16 / sizeof(T);
+  if (wide) {
+    constexpr uint32_t kPer = kD / N;
+    for (uint32_t i = threadIdx.x; i < ROWS * kPer; i += kThreads) {
+      const uint32_t r = i / kPer, c = (i % kPer) * N, row = row0 + r;
+      const T *from = base;
+      uint32_t bytes = 0;
+      if (row < rows && c < head) {
+        const uint32_t tok = per == 1u ? row : row / per;
+        from = base + tok * ld + static_cast<unsigned long long>(row - tok * per) * head + c;
+        bytes = 16;
+      }
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at(dst + r * P + c)), "l"(from), "r"(bytes) : "memory");
+    }
+  } else {
+    for (uint32_t i = threadIdx.x; i < ROWS * kD; i += kThreads) {
+      const uint32_t r = i / kD, c = i % kD, row = row0 + r;
+      T v = T(0.f);
+      if (row < rows && c < head) {
+        const uint32_t tok = per == 1u ? row : row / per;
+        v = base[tok * ld + static_cast<unsigned long long>(row - tok * per) * head + c];
+      }
+      dst[r * P + c] = v;
+    }
+  }
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T> __device__ __forceinline__ T round_to(float v);
+template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+
+// One row's columns of an accumulator: columns col0 + 8n + 2t, + 1.
+template <typename T, int kCols>
+__device__ __forceinline__ void store_row(T *out, const float (&acc)[kCols / 8][4], int half, int col0, uint32_t head, float factor, int accumulate) {
+  const uint32_t t = threadIdx.x & 3u;
+#pragma unroll
+  for (int n = 0; n < kCols / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t c = col0 + n * 8 + 2 * t + e;
+      if (c < head) {
+        float v = acc[n][half * 2 + e] * factor;
+        if (accumulate) v += static_cast<float>(out[c]);
+        out[c] = round_to<T>(v);
+      }
+    }
+}
+
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+template <typename T> __device__ __forceinline__ float exp2_of(float x) {
+  if constexpr (sizeof(T) == 2) return attn_exp2(x);
+  else return exp2f(x);
+}
+
+enum { kWideQ = 1, kWideK = 2, kWideV = 4, kWideGy = 8 };
+
+// ---- forward ---------------------------------------------------------------------------------------------
+
+template <typename T, int kD> constexpr int kFwCols = sizeof(T) == 2 ? 64 : 32;
+
+template <typename T, int kD, int kPass>
+__global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t tiles, int wide) {
+  pdl_enter();
+  constexpr int BN = kFwCols<T, kD>, NT = BN / 8, P = kPitch<T, kD>;
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  __shared__ uint32_t s_at[2];
+  T *sq = reinterpret_cast<T *>(s_raw), *sk = sq + kRows * P, *sv = sk + 2 * BN * P;
+  // the last tiles of a causal sequence have the most keys: they go first
+  uint32_t seq, tile;
+  if (!attn_find_tile<false>(a, tiles - 1u - blockIdx.x, a.group, kRows, s_at, seq, tile)) return;
+  const AttnSeq q = attn_seq(a, seq);
+  const uint32_t hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+  const uint32_t rows = q.lq * a.group, row0 = tile * kRows;
+  const T *qb = static_cast<const T *>(a.q) + q.q0 * a.q_ld + static_cast<unsigned long long>(hk) * a.group * a.head;
+  const T *kb = static_cast<const T *>(a.k) + q.k0 * a.k_ld + static_cast<unsigned long long>(hk) * a.head;
+  const T *vb = static_cast<const T *>(a.v) + q.k0 * a.v_ld + static_cast<unsigned long long>(hk) * a.head;
+  const long long shift = static_cast<long long>(q.lk) - q.lq;   // query i sees keys up to i + shift
+  uint32_t keys = q.lk;
+  if (a.causal) {
+    const long long seen = static_cast<long long>((min(row0 + kRows, rows) - 1u) / a.group) + shift + 1;
+    keys = seen <= 0 ? 0u : min(keys, static_cast<uint32_t>(seen));
+  }
+  const uint32_t steps = (keys + BN - 1) / BN;
+
+  load_rows<T, kD, kRows, 128>(sq, qb, a.q_ld, a.group, row0, rows, a.head, wide & kWideQ);
+  if (steps) {
+    load_rows<T, kD, BN, 128>(sk, kb, a.k_ld, 1, 0, keys, a.head, wide & kWideK);
+    load_rows<T, kD, BN, 128>(sv, vb, a.v_ld, 1, 0, keys, a.head, wide & kWideV);
+  }
+  copies_commit();
+
+  uint32_t row[2];
+  long long last[2];       // the last key that each of this lane's two rows sees
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    row[r] = row0 + warp * 16 + g + r * 8;
+    last[r] = row[r] >= rows ? -1 : (a.causal ? static_cast<long long>(row[r] / a.group) + shift : static_cast<long long>(q.lk) - 1);
+  }
+  float acc[kD / 8][4];
+#pragma unroll
+  for (int n = 0; n < kD / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+  const float to2 = a.scale * kLog2e;
+
+  for (uint32_t step = 0; step < steps; ++step) {
+    const uint32_t at = step & 1u;
+    copies_wait<0>();
+    __syncthreads();
+    if (step + 1 < steps) {
+      const uint32_t next = (step + 1) * BN;
+      load_rows<T, kD, BN, 128>(sk + (at ^ 1u) * BN * P, kb, a.k_ld, 1, next, keys, a.head, wide & kWideK);
+      load_rows<T, kD, BN, 128>(sv + (at ^ 1u) * BN * P, vb, a.v_ld, 1, next, keys, a.head, wide & kWideV);
+      copies_commit();
+    }
+    float s[NT][4];
+    product_abt<kD, NT, kPass>(s, sq + warp * 16 * P, sk + at * BN * P);
+    const uint32_t key0 = step * BN;
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool seen = static_cast<long long>(key0 + n * 8 + 2 * t + (i & 1)) <= last[i >> 1];
+        s[n][i] = seen ? s[n][i] * to2 : -INFINITY;
+        top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
+      }
+    float keep[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float now = fmaxf(m[r], quad_max(top[r]));
+      const float base = now == -INFINITY ? 0.f : now;   // nothing seen yet: every p below is exp2(-inf)
+      keep[r] = exp2_of<T>(m[r] - base);
+      m[r] = now;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p = exp2_of<T>(s[n][r * 2 + e] - base);
+          s[n][r * 2 + e] = p;
+          sum += p;
+        }
+      l[r] = l[r] * keep[r] + sum;
+    }
+    product_py<kD, kD, NT, kPass>(acc, s, sv + at * BN * P, 0, keep[0], keep[1]);
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] = quad_sum(l[r]);
+    if (row[r] >= rows) continue;
+    const uint32_t tok = row[r] / a.group, h = hk * a.group + row[r] - tok * a.group;
+    const bool any = m[r] != -INFINITY;
+    store_row<T, kD>(static_cast<T *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(h) * a.head, acc, r, 0, a.head,
+                     any ? 1.f / l[r] : 0.f, 0);
+    if (a.lse && t == 0) a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = any ? m[r] * kLn2 + logf(l[r]) : -INFINITY;
+  }
+}
+
+// ---- backward ----------------------------------------------------------------------------------------------
+
+template <typename T, int kD> constexpr int kBwCols = sizeof(T) == 2 && kD == 64 ? 64 : 32;
+template <typename T, int kD> constexpr int kBwThreads = kD == 256 ? 256 : 128;   // 256 columns: a warp has half of them
+template <typename T, int kD> constexpr int kBwStages = sizeof(T) == 4 && kD == 256 ? 1 : 2;
+
+// The power of two that takes the largest |ds| possible to at most 2^14.  |dp - delta| <= |gy| |v| + |delta|.
+__device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) {
+  const float bound = sqrtf(gy_sq) * sqrtf(v_sq) + delta;
+  if (!(bound > 1e-30f) || !(bound < 1e30f)) return 1.f;
+  return exp2f(fminf(fmaxf(13.f - ceilf(log2f(bound)), -100.f), 100.f));
+}
+
+// kKeys: the keys rest, the queries of all heads of the group pass by (gk, gv).  Else the queries rest (gq).
+template <typename T, int kD, int kPass, bool kKeys>
+__global__ void __launch_bounds__(kBwThreads<T, kD>) attention_bw_kernel(AttnArgs a, uint32_t tiles, int wide) {
+  pdl_enter();
+  constexpr int BN = kBwCols<T, kD>, NT = BN / 8, P = kPitch<T, kD>, kThreads = kBwThreads<T, kD>, kStages = kBwStages<T, kD>;
+  constexpr int kCols = kD == 256 ? 128 : kD;
+  constexpr bool kHalf = sizeof(T) == 2;
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  __shared__ uint32_t s_at[2];
+  __shared__ float s_lse[2][BN], s_delta[2][BN], s_max[3][8];
+  T *x1 = reinterpret_cast<T *>(s_raw), *x2 = x1 + kRows * P, *y1 = x2 + kRows * P, *y2 = y1 + kStages * BN * P;
+  uint32_t seq, tile;
+  if (!attn_find_tile<kKeys>(a, kKeys ? blockIdx.x : tiles - 1u - blockIdx.x, kKeys ? 1u : a.group, kRows, s_at, seq, tile)) return;
+  const AttnSeq q = attn_seq(a, seq);
+  const uint32_t hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+  const uint32_t wrow = (warp & 3u) * 16u, col0 = (warp >> 2) * kCols;
+  const uint32_t qrows = q.lq * a.group, row0 = tile * kRows, rows = kKeys ? q.lk : qrows;
+  const unsigned long long hq_at = static_cast<unsigned long long>(hk) * a.group * a.head, hk_at = static_cast<unsigned long long>(hk) * a.head;
+  const T *qb = static_cast<const T *>(a.q) + q.q0 * a.q_ld + hq_at, *gyb = static_cast<const T *>(a.gy) + q.q0 * a.y_ld + hq_at;
+  const T *kb = static_cast<const T *>(a.k) + q.k0 * a.k_ld + hk_at, *vb = static_cast<const T *>(a.v) + q.k0 * a.v_ld + hk_at;
+  const long long shift = static_cast<long long>(q.lk) - q.lq;
+  // what passes by: queries from the first that sees a key of the tile, or keys up to the last that a query of the tile sees
+  uint32_t from = 0, to = kKeys ? qrows : q.lk;
+  if (a.causal) {
+    if (kKeys) {
+      const long long first = static_cast<long long>(row0) - shift;
+      from = first <= 0 ? 0u : (first >= q.lq ? qrows : static_cast<uint32_t>(first) * a.group);
+    } else {
+      const long long seen = static_cast<long long>((min(row0 + kRows, rows) - 1u) / a.group) + shift + 1;
+      to = seen <= 0 ? 0u : min(to, static_cast<uint32_t>(seen));
+    }
+  }
+  const uint32_t steps = to > from ? (to - from + BN - 1) / BN : 0u;
+  const unsigned long long stat = static_cast<unsigned long long>(hk) * a.group * a.rows_q + q.q0;   // of query 0, first head
+
+  auto load_step = [&](uint32_t step, uint32_t at) {
+    const uint32_t r0 = from + step * BN;
+    if constexpr (kKeys) {
+      load_rows<T, kD, BN, kThreads>(y1 + at * BN * P, qb, a.q_ld, a.group, r0, to, a.head, wide & kWideQ);
+      load_rows<T, kD, BN, kThreads>(y2 + at * BN * P, gyb, a.y_ld, a.group, r0, to, a.head, wide & kWideGy);
+      if (threadIdx.x < BN) {
+        const uint32_t r = r0 + threadIdx.x, tok = r / a.group;
+        const unsigned long long i = stat + static_cast<unsigned long long>(r - tok * a.group) * a.rows_q + tok;
+        s_lse[at][threadIdx.x] = r < to ? a.lse[i] * kLog2e : 0.f;
+        s_delta[at][threadIdx.x] = r < to ? a.delta[i] : 0.f;
+      }
+    } else {
+      load_rows<T, kD, BN, kThreads>(y1 + at * BN * P, kb, a.k_ld, 1, r0, to, a.head, wide & kWideK);
+      load_rows<T, kD, BN, kThreads>(y2 + at * BN * P, vb, a.v_ld, 1, r0, to, a.head, wide & kWideV);
+    }
+    copies_commit();
+  };
+  if constexpr (kKeys) {
+    load_rows<T, kD, kRows, kThreads>(x1, kb, a.k_ld, 1, row0, rows, a.head, wide & kWideK);
+    load_rows<T, kD, kRows, kThreads>(x2, vb, a.v_ld, 1, row0, rows, a.head, wide & kWideV);
+  } else {
+    load_rows<T, kD, kRows, kThreads>(x1, qb, a.q_ld, a.group, row0, rows, a.head, wide & kWideQ);
+    load_rows<T, kD, kRows, kThreads>(x2, gyb, a.y_ld, a.group, row0, rows, a.head, wide & kWideGy);
+  }
+  if (steps) load_step(0, 0);
+  else copies_commit();
+
+  float ds_scale = 1.f;
+  if constexpr (kHalf) {   // over all that this block sees: the scale must not change on the way
+    const uint32_t q_from = kKeys ? from : row0, q_to = kKeys ? qrows : min(row0 + kRows, rows);
+    const uint32_t k_from = kKeys ? row0 : 0u, k_to = kKeys ? min(row0 + kRows, rows) : to;
+    float gm = 0.f, dm = 0.f, vm = 0.f;
+    for (uint32_t r = q_from + threadIdx.x; r < q_to; r += kThreads) {
+      const uint32_t tok = r / a.group;
+      const unsigned long long i = stat + static_cast<unsigned long long>(r - tok * a.group) * a.rows_q + tok;
+      gm = fmaxf(gm, a.gy_norm[i]);
+      dm = fmaxf(dm, fabsf(a.delta[i]));
+    }
+    for (uint32_t r = k_from + threadIdx.x; r < k_to; r += kThreads)
+      vm = fmaxf(vm, a.v_norm[static_cast<unsigned long long>(hk) * a.rows_k + q.k0 + r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+      dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, o));
+      vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+    }
+    if (lane == 0) s_max[0][warp] = gm, s_max[1][warp] = dm, s_max[2][warp] = vm;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 32; ++w) gm = fmaxf(gm, s_max[0][w]), dm = fmaxf(dm, s_max[1][w]), vm = fmaxf(vm, s_max[2][w]);
+    ds_scale = scale_of(gm, vm, dm);
+  }
+
+  uint32_t row[2];
+  float row_lse[2] = {0.f, 0.f}, row_delta[2] = {0.f, 0.f};
+  unsigned long long row_at[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    row[r] = row0 + wrow + g + r * 8;
+    const uint32_t tok = row[r] / a.group;
+    row_at[r] = stat + static_cast<unsigned long long>(row[r] - tok * a.group) * a.rows_q + tok;
+    if (!kKeys && row[r] < rows) {
+      row_lse[r] = a.lse[row_at[r]] * kLog2e;
+      row_delta[r] = a.delta[row_at[r]];
+    }
+  }
+  float acc1[kKeys ? kCols / 8 : 1][4], acc2[kCols / 8][4];
+#pragma unroll
+  for (int n = 0; n < kCols / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc2[n][i] = 0.f;
+      if constexpr (kKeys) acc1[n][i] = 0.f;
+    }
+  const float to2 = a.scale * kLog2e;
+
+  for (uint32_t step = 0; step < steps; ++step) {
+    const uint32_t at = kStages == 2 ? step & 1u : 0u;
+    if (kStages == 1 && step > 0) {
+      __syncthreads();
+      load_step(step, 0);
+    }
+    copies_wait<0>();
+    __syncthreads();
+    if (kStages == 2 && step + 1 < steps) load_step(step + 1, at ^ 1u);
+    float p[NT][4], ds[NT][4];
+    product_abt<kD, NT, kPass>(p, x1 + wrow * P, y1 + at * BN * P);
+    product_abt<kD, NT, kPass>(ds, x2 + wrow * P, y2 + at * BN * P);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t c = n * 8 + 2 * t + (i & 1), col = from + step * BN + c, r = row[i >> 1];
+        const uint32_t key = kKeys ? r : col, qr = kKeys ? col : r;
+        const bool seen = key < q.lk && qr < qrows && (!a.causal || static_cast<long long>(key) <= static_cast<long long>(qr / a.group) + shift);
+        const float lse = kKeys ? s_lse[at][c] : row_lse[i >> 1], delta = kKeys ? s_delta[at][c] : row_delta[i >> 1];
+        const float e = seen ? exp2_of<T>(p[n][i] * to2 - lse) : 0.f;
+        ds[n][i] = seen ? e * (ds[n][i] - delta) * ds_scale : 0.f;
+        p[n][i] = kHalf ? e * kPScale : e;
+      }
+    if constexpr (kKeys) product_py<kD, kCols, NT, kPass>(acc1, p, y2 + at * BN * P, col0, 1.f, 1.f);
+    product_py<kD, kCols, NT, kPass>(acc2, ds, y1 + at * BN * P, col0, 1.f, 1.f);
+  }
+  const float undo = a.scale / ds_scale;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    if (row[r] >= rows) continue;
+    if constexpr (kKeys) {
+      store_row<T, kCols>(static_cast<T *>(a.gv) + (q.k0 + row[r]) * a.v_ld + hk_at, acc1, r, col0, a.head, kHalf ? 1.f / kPScale : 1.f, a.accumulate);
+      store_row<T, kCols>(static_cast<T *>(a.gk) + (q.k0 + row[r]) * a.k_ld + hk_at, acc2, r, col0, a.head, undo, a.accumulate);
+    } else {
+      const uint32_t tok = row[r] / a.group;
+      store_row<T, kCols>(static_cast<T *>(a.gq) + (q.q0 + tok) * a.q_ld + hq_at + static_cast<unsigned long long>(row[r] - tok * a.group) * a.head,
+                          acc2, r, col0, a.head, undo, a.accumulate);
+    }
+  }
+}
+
+// ---- launches ----------------------------------------------------------------------------------------------
+
+int find_wide(const AttnArgs &a, size_t es) {
+  auto ok = [&](const void *p, unsigned long long ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0 && a.head * es % 16 == 0;
+  };
+  return (ok(a.q, a.q_ld) ? kWideQ : 0) | (ok(a.k, a.k_ld) ? kWideK : 0) | (ok(a.v, a.v_ld) ? kWideV : 0) | (ok(a.gy, a.y_ld) ? kWideGy : 0);
+}
+
+// cudaFuncSetAttribute once per kernel and device would do; it is cheap beside a launch and needs no state.
+template <typename K>
+int allow_smem(K kernel, size_t smem) {
+  return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+}
+
+template <typename T, int kD, int kPass>
+int launch_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
+  constexpr size_t smem = sizeof(T) * kPitch<T, kD> * (kRows + 4 * kFwCols<T, kD>);
+  const uint32_t tiles = static_cast<uint32_t>(attn_tile_bound(a.rows_q, a.max_q, a.seqs, a.group, kRows));
+  auto kernel = attention_fw_kernel<T, kD, kPass>;
+  if (const int rc = allow_smem(kernel, smem)) return rc;
+  b200::launch(ctx, kernel, dim3(tiles, a.heads_k), dim3(128), smem, s, 1u, a, tiles, find_wide(a, sizeof(T)));
+  return B200_OK;
+}
+
+template <typename T, int kD, int kPass, bool kKeys>
+int launch_bw_side(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
+  constexpr size_t smem = sizeof(T) * kPitch<T, kD> * (2 * kRows + 2 * kBwStages<T, kD> * kBwCols<T, kD>);
+  const uint32_t tiles = static_cast<uint32_t>(kKeys ? attn_tile_bound(a.rows_k, a.max_k, a.seqs, 1, kRows)
+                                                     : attn_tile_bound(a.rows_q, a.max_q, a.seqs, a.group, kRows));
+  if (tiles == 0) return B200_OK;
+  auto kernel = attention_bw_kernel<T, kD, kPass, kKeys>;
+  if (const int rc = allow_smem(kernel, smem)) return rc;
+  b200::launch(ctx, kernel, dim3(tiles, a.heads_k), dim3(kBwThreads<T, kD>), smem, s, 1u, a, tiles, find_wide(a, sizeof(T)));
+  ++ctx->launches;
+  return B200_OK;
+}
+
+template <typename T, int kPass, typename F>
+int with_head(uint32_t head, F f) {
+  if (head <= 64) return f(std::integral_constant<int, 64>());
+  if (head <= 128) return f(std::integral_constant<int, 128>());
+  return f(std::integral_constant<int, 256>());
+}
+
+template <typename F>
+int with_type(int mode, F f) {
+  if (mode == B200_MODE_FP16) return f(__half(), std::integral_constant<int, 1>());
+  if (mode == B200_MODE_TF32) return f(float(), std::integral_constant<int, 1>());
+  return f(float(), std::integral_constant<int, 3>());
+}
+
+}  // namespace
+
+int attention_mma_fw(b200_ctx *ctx, int mode, const AttnArgs &a, cudaStream_t s) {
+  return with_type(mode, [&](auto type, auto pass) {
+    using T = decltype(type);
+    return with_head<T, decltype(pass)::value>(a.head, [&](auto d) { return launch_fw<T, decltype(d)::value, decltype(pass)::value>(ctx, a, s); });
+  });
+}
+
+int attention_mma_bw(b200_ctx *ctx, int mode, const AttnArgs &a, cudaStream_t s) {
+  return with_type(mode, [&](auto type, auto pass) {
+    using T = decltype(type);
+    return with_head<T, decltype(pass)::value>(a.head, [&](auto d) {
+      constexpr int kD = decltype(d)::value, kPass = decltype(pass)::value;
+      if (const int rc = launch_bw_side<T, kD, kPass, true>(ctx, a, s)) return rc;
+      if (const int rc = launch_bw_side<T, kD, kPass, false>(ctx, a, s)) return rc;
+      --ctx->launches;   // the entry point counts the last one
+      return static_cast<int>(B200_OK);
+    });
+  });
+}
+
+}  // namespace b200
