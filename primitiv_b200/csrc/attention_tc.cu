@@ -1,0 +1,449 @@
+// Attention of halves on the tcgen05 tensor cores, for heads of up to 128 elements that TMA can address.
+//
+// Forward.  A block has two tiles of 128 queries that share their keys: two heads of one group where the group is
+// even, else 256 queries of one head.  Warps 0-3 and 4-7 are the softmax of one tile each, a thread a row; warp 8
+// issues every matrix instruction, warp 9 every copy.  Keys and values come through one ring of 128-row tiles.
+//   tensor memory: s of tile 0, s of tile 1 (128 columns each), y of tile 0, y of tile 1
+//   p is written over s as halves, and is the left operand of p v from there: it never passes through shared memory
+// While one tile's rows are in their softmax, the tensor core has the other tile's two products: per 128 keys of one tile
+// 1024 clocks of matrix instructions stand against 16384 exponentials, which are 1024 clocks of the special function
+// units.  The products run in the order in which they were issued, so p(j) v is read before s(j + 1) overwrites it.
+//
+// The running maximum that scales y is only moved when a row has passed it by more than 2^8: until then p may exceed one (at most
+// 256, exact enough in halves), and y stays in tensor memory untouched.  Moving it costs a pass over y, by the softmax
+// warps themselves, a few times per row.
+//
+// Every wait is bounded, as in gemm_tc.cu.
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "attention.h"
+#include "tcgen05.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr uint32_t kTile = 128;                      // queries and keys of a tile
+constexpr uint32_t kChunk = kTile * 128;             // bytes of 64 columns of a tile: 128-byte lines, swizzled
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// ---- matrix instructions ------------------------------------------------------------------------------------
+
+// Left operand from tensor memory.  All lanes of a converged warp, uniform arguments.
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, e;\n\t"
+      ".reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t"
+      "}\n" ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// fp32 accumulator, both operands halves, M = 128, N columns; `mn`: the right operand lies N-major (its rows are k).
+constexpr uint32_t idesc_of(uint32_t n, uint32_t mn) { return (1u << 4) | (mn << 16) | ((n >> 3) << 17) | ((kTile >> 4) << 24); }
+// 128-byte swizzle, groups of eight lines 1024 bytes apart
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+// d[128][128 or N] = A . B^T over kD columns, both tiles of 128-byte lines in chunks of 64 columns.
+template <int kD>
+__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+  for (int c = 0; c < kD / 64; ++c)
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const uint32_t at = c * kChunk + ks * 32;
+      mma_issue<1, true>(d, ((a + at) & 0x3FFFFu) >> 4, kDescHi, ((b + at) & 0x3FFFFu) >> 4, kDescHi, idesc, (c | ks) != 0);
+    }
+}
+// d[128][kD] (+)= P . B, P of 128 halves a row in tensor memory, B a tile of 128 rows.
+__device__ __forceinline__ void product_pn(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks)
+    mma_from_tmem(d, p + ks * 8, (((b + ks * 2048) & 0x3FFFFu) >> 4) | ((kChunk >> 4) << 16), kDescHi, idesc, !(first && ks == 0));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- pairs of floats ----------------------------------------------------------------------------------------
+
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t halves_of(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// All lanes of the warp.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------
+
+struct alignas(64) FwParams {
+  CUtensorMap q, k, v;
+  AttnArgs a;
+  uint32_t tiles, columns;   // tiles of all sequences (a bound); blocks per tile: heads, or pairs of them
+  uint32_t two_heads;        // a block's two tiles are two heads; else 256 queries of one
+  int *status;
+};
+
+constexpr uint32_t kFwThreads = 384;   // three warps on each quarter of an SM; the last two only lend their registers
+
+template <int kD> constexpr uint32_t kFwStages = kD == 128 ? 5u : 8u;
+template <int kD> constexpr uint32_t kFwSmem = (2 + kFwStages<kD>) * kTile * kD * 2 + 1024;
+
+template <int kD>
+__global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __grid_constant__ FwParams p) {
+  constexpr uint32_t kBytes = kTile * kD * 2, kStages = kFwStages<kD>, kChunks = kD / 64;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t q_full, full_bar[kStages], empty_bar[kStages], s_full[2], p_full[2], y_done[2], v_clean, drain_bar;
+  __shared__ uint32_t tmem_slot, s_at[2];
+  __shared__ int s_abort;
+  pdl_release_next();
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem + 2 * kBytes;
+  volatile int *abort_flag = &s_abort;
+  const AttnArgs &a = p.a;
+  if (threadIdx.x == 9u * 32u) {
+    for (const CUtensorMap *m : {&p.q, &p.k, &p.v}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(m)) : "memory");
+  }
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    mbar_init(smem_u32(&q_full), 1);
+    for (uint32_t i = 0; i < kStages; ++i) mbar_init(smem_u32(&full_bar[i]), 1), mbar_init(smem_u32(&empty_bar[i]), 1);
+    for (uint32_t x = 0; x < 2; ++x) mbar_init(smem_u32(&s_full[x]), 1), mbar_init(smem_u32(&p_full[x]), 4), mbar_init(smem_u32(&y_done[x]), 1);
+    mbar_init(smem_u32(&v_clean), 1);
+    mbar_init(smem_u32(&drain_bar), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait_previous();
+  tc_fence_before();
+  // the last tiles of a causal sequence have the most keys: they go first
+  const uint32_t column = blockIdx.x % p.columns, unit = p.two_heads ? kTile : 2 * kTile;
+  uint32_t seq, tile;
+  const bool any = attn_find_tile<false>(a, p.tiles - 1u - blockIdx.x / p.columns, 1, unit, s_at, seq, tile);
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (any) {
+    const AttnSeq q = attn_seq(a, seq);
+    const long long shift = static_cast<long long>(q.lk) - q.lq;
+    const uint32_t head0 = p.two_heads ? 2 * column : column, kv_head = head0 / a.group;
+    uint32_t tok0[2], tiles[2], keys = 0, steps = 0;
+    bool has[2];
+#pragma unroll
+    for (uint32_t x = 0; x < 2; ++x) {
+      tok0[x] = tile * unit + (p.two_heads ? 0u : x * kTile);
+      has[x] = tok0[x] < q.lq;
+      uint32_t n = q.lk;
+      if (a.causal) {
+        const long long seen = static_cast<long long>(min(tok0[x] + kTile, q.lq)) + shift;
+        n = seen <= 0 ? 0u : min(n, static_cast<uint32_t>(seen));
+      }
+      tiles[x] = has[x] ? (n + kTile - 1) / kTile : 0u;
+      if (has[x]) keys = max(keys, n);
+      steps = max(steps, tiles[x]);
+    }
+    const uint32_t left = keys % kTile;   // keys in the last tile, 0 = all
+
+    // 168 registers a thread at launch: 56 + 2 * 224 = 3 * 168
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 9) {
+      // ------------------------------ copies ------------------------------
+      if (steps > 0) {
+        uint32_t stage = 0, phase = 0, armed = 0, parity = 0;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(smem_u32(&q_full), ((has[0] ? 1u : 0u) + (has[1] ? 1u : 0u)) * kBytes);
+          for (uint32_t x = 0; x < 2; ++x)
+            for (uint32_t c = 0; c < kChunks; ++c)
+              if (has[x]) tma_load_3d(smem + x * kBytes + c * kChunk, &p.q, smem_u32(&q_full), c * 64, head0 + (p.two_heads ? x : 0u), q.q0 + tok0[x]);
+        }
+        __syncwarp();
+        bool ok = true;
+        uint32_t last_bar = 0, last_parity = 0, last_at = 0;
+        for (uint32_t i = 0; ok && i < 2 * steps; ++i) {   // keys, values, keys, values, ...
+          if (!wait_all(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = smem_u32(&full_bar[stage]), dst = ring + stage * kBytes;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar, kBytes);
+            for (uint32_t c = 0; c < kChunks; ++c) tma_load_3d(dst + c * kChunk, (i & 1u) ? &p.v : &p.k, bar, c * 64, kv_head, q.k0 + (i >> 1) * kTile);
+          }
+          __syncwarp();
+          armed |= 1u << stage;
+          parity = (parity & ~(1u << stage)) | (phase << stage);
+          last_bar = bar, last_parity = phase, last_at = dst;
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+        // The last tile of values: rows behind the last key hold another sequence's, or anything; p is zero there, but zero
+        // times an infinity is not.
+        if (ok && left != 0u && wait_all(last_bar, last_parity, abort_flag)) {
+          for (uint32_t c = 0; c < kChunks; ++c)
+            for (uint32_t at = left * 128u + lane * 16u; at < kChunk; at += 512u)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(last_at + c * kChunk + at), "r"(0u) : "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&v_clean));
+        }
+        if (*abort_flag) {   // the copies in flight land before shared memory is given up
+          mbar_wait_quiet(smem_u32(&q_full), 0);
+          for (uint32_t s = 0; s < kStages; ++s)
+            if (armed & (1u << s)) mbar_wait_quiet(smem_u32(&full_bar[s]), (parity >> s) & 1u);
+        }
+      }
+    } else if (warp == 8) {
+      // ------------------------------ products ------------------------------
+      if (steps > 0) {
+        constexpr uint32_t kS = idesc_of(kTile, 0), kY = idesc_of(kD, 1);
+        uint32_t stage = 0, phase = 0;
+        bool ok = wait_all(smem_u32(&q_full), 0, abort_flag) && wait_all(smem_u32(&full_bar[0]), 0, abort_flag);
+        if (ok) {
+#pragma unroll
+          for (uint32_t x = 0; x < 2; ++x)
+            if (tiles[x] > 0) {
+              product_nt<kD>(tmem + x * kTile, smem + x * kBytes, ring, kS);
+              mma_commit(smem_u32(&s_full[x]));
+            }
+          mma_commit(smem_u32(&empty_bar[0]));
+          stage = 1;
+        }
+        for (uint32_t j = 0; ok && j < steps; ++j) {
+          const uint32_t v_stage = stage, v_phase = phase;
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+          const uint32_t k_stage = stage;
+          if (!wait_all(smem_u32(&full_bar[v_stage]), v_phase, abort_flag)) { ok = false; break; }
+          if (j + 1 == steps && left != 0u && !wait_all(smem_u32(&v_clean), 0, abort_flag)) { ok = false; break; }
+          if (j + 1 < steps && !wait_all(smem_u32(&full_bar[k_stage]), phase, abort_flag)) { ok = false; break; }
+#pragma unroll
+          for (uint32_t x = 0; x < 2; ++x) {
+            if (ok && j < tiles[x]) {
+              if (!wait_all(smem_u32(&p_full[x]), j & 1u, abort_flag)) {
+                ok = false;
+              } else {
+                tc_fence_after();
+                product_pn(tmem + 2 * kTile + x * kD, tmem + x * kTile, ring + v_stage * kBytes, kY, j == 0);
+                mma_commit(smem_u32(&y_done[x]));
+                if (j + 1 < tiles[x]) {
+                  product_nt<kD>(tmem + x * kTile, smem + x * kBytes, ring + k_stage * kBytes, kS);
+                  mma_commit(smem_u32(&s_full[x]));
+                }
+              }
+            }
+          }
+          if (!ok) break;
+          mma_commit(smem_u32(&empty_bar[v_stage]));
+          if (j + 1 < steps) {
+            mma_commit(smem_u32(&empty_bar[k_stage]));
+            if (++stage == kStages) stage = 0, phase ^= 1u;
+          }
+        }
+        if (*abort_flag) {   // retire whatever was issued before tensor memory is freed
+          __syncwarp();
+          mma_commit(smem_u32(&drain_bar));
+          mbar_wait_quiet(smem_u32(&drain_bar), 0);
+        }
+      }
+    } else if (warp < 8) {
+      // ------------------------------ softmax ------------------------------
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+      const uint32_t x = warp >> 2, quarter = warp & 3u;
+      const uint32_t lanes = (quarter * 32u) << 16, s_tmem = tmem + lanes + x * kTile, y_tmem = tmem + lanes + 2 * kTile + x * kD;
+      const uint32_t tok = (x ? tok0[1] : tok0[0]) + quarter * 32u + lane, n = x ? tiles[1] : tiles[0];
+      // keys that this row sees
+      long long sees = q.lk;
+      if (a.causal) sees = min(sees, max(0ll, static_cast<long long>(tok) + 1 + shift));
+      const float to2 = a.scale * kLog2e;
+      float m = -INFINITY, l = 0.f;     // maximum in units of s, and the sum at that maximum
+      bool ok = true;
+      for (uint32_t j = 0; j < n; ++j) {
+        if (!wait_all(smem_u32(&s_full[x]), j & 1u, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_issue(s_tmem + c * 32, s[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait(s[c]);
+        const int seen = static_cast<int>(max(-1ll, min(sees - static_cast<long long>(j) * kTile, static_cast<long long>(kTile))));
+        if (__any_sync(0xffffffffu, seen < static_cast<int>(kTile))) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= seen) s[c][i] = 0xff800000u;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[c][i]));
+        const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        // (a row that has seen nothing has m = -inf: its sum and y are zeros, whatever they are multiplied with)
+        const bool move = now > m && (now - m) * to2 > 8.f;
+        if (j == 0) {
+          m = now;
+        } else if (__any_sync(0xffffffffu, move)) {
+          const float keep = move ? attn_exp2((m - now) * to2) : 1.f;
+          if (move) m = now;
+          l *= keep;
+          if (!wait_all(smem_u32(&y_done[x]), (j - 1) & 1u, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < kD / 32; ++c) {
+            uint32_t y[32];
+            tmem_ld32(y_tmem + c * 32, y);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
+            tmem_st32(y_tmem + c * 32, y);
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : -m * to2;
+        const f32x2 to22 = pair_of(to2, to2), base2 = pair_of(base, base);
+        f32x2 sum[2] = {0ull, 0ull};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t out[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int c = h * 2 + i / 16, e = (i % 16) * 2;
+            float u, w;
+            unpair(fma2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), to22, base2), u, w);
+            u = attn_exp2(u), w = attn_exp2(w);
+            sum[i & 1] = add2(sum[i & 1], pair_of(u, w));
+            out[i] = halves_of(u, w);
+          }
+          tmem_st32(s_tmem + h * 32, out);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&p_full[x]));
+        float u, w;
+        unpair(add2(sum[0], sum[1]), u, w);
+        l += u + w;
+      }
+      if (ok && n > 0) ok = wait_all(smem_u32(&y_done[x]), (n - 1) & 1u, abort_flag);
+      tc_fence_after();
+      if (ok && (x ? has[1] : has[0])) {
+        const bool some = m != -INFINITY, mine = tok < q.lq;
+        const float inv = some ? 1.f / l : 0.f;
+        const uint32_t head = head0 + (p.two_heads ? x : 0u);
+        __half *out = static_cast<__half *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(head) * a.head;
+#pragma unroll
+        for (int c = 0; c < kD / 32; ++c) {
+          uint32_t y[32];
+          if (n > 0) tmem_ld32(y_tmem + c * 32, y);
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            if (mine && c * 32 + i < a.head) {
+              uint4 o = make_uint4(0u, 0u, 0u, 0u);
+              if (some) {
+                o.x = halves_of(__uint_as_float(y[i]) * inv, __uint_as_float(y[i + 1]) * inv);
+                o.y = halves_of(__uint_as_float(y[i + 2]) * inv, __uint_as_float(y[i + 3]) * inv);
+                o.z = halves_of(__uint_as_float(y[i + 4]) * inv, __uint_as_float(y[i + 5]) * inv);
+                o.w = halves_of(__uint_as_float(y[i + 6]) * inv, __uint_as_float(y[i + 7]) * inv);
+              }
+              *reinterpret_cast<uint4 *>(out + c * 32 + i) = o;
+            }
+          }
+        }
+        if (a.lse && mine) a.lse[static_cast<unsigned long long>(head) * a.rows_q + q.q0 + tok] = some ? m * to2 * kLn2 + logf(l) : -INFINITY;
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && s_abort) report_status(p.status, B200_ERR_KERNEL_TIMEOUT);
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------
+
+// Shape({head, heads, rows}) in boxes of 64 elements of one head of 128 rows; what lies past the head or the rows reads as zero.
+int encode(const b200_ctx *ctx, CUtensorMap *map, const void *p, uint32_t head, uint32_t heads, uint32_t rows, unsigned long long ld) {
+  cuuint64_t dims[3] = {head, heads, rows}, strides[2] = {head * 2ull, ld * 2ull};
+  cuuint32_t box[3] = {64, 1, kTile}, step[3] = {1, 1, 1};
+  const CUresult r = ctx->encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(p), dims, strides, box, step,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200_OK : B200_ERR_DRIVER;
+}
+
+bool addressable(const void *p, unsigned long long ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld * 2 < (1ull << 40); }
+
+template <int kD>
+int launch_fw(b200_ctx *ctx, const FwParams &p, cudaStream_t s) {
+  auto kernel = attention_fw_tc_kernel<kD>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kFwSmem<kD>));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  b200::launch(ctx, kernel, dim3(p.tiles * p.columns), dim3(kFwThreads), kFwSmem<kD>, s, 1u, p);
+  return B200_OK;
+}
+
+}  // namespace
+
+bool attention_tc_fw_eligible(const b200_ctx *ctx, int mode, const AttnArgs &a) {
+  return mode == B200_MODE_FP16 && ctx->encode_tiled && a.head <= 128 && a.head % 8 == 0 && a.scale > 0.f && a.max_k > 0 &&
+         addressable(a.q, a.q_ld) && addressable(a.k, a.k_ld) && addressable(a.v, a.v_ld) && addressable(a.y, a.y_ld);
+}
+
+int attention_tc_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
+  FwParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.a = a;
+  p.two_heads = a.group % 2 == 0;
+  p.columns = p.two_heads ? a.heads_q / 2 : a.heads_q;
+  const unsigned long long tiles = attn_tile_bound(a.rows_q, a.max_q, a.seqs, 1, p.two_heads ? kTile : 2 * kTile);
+  if (tiles * p.columns > 0x7fffffffull) return B200_ERR_TOO_LARGE;
+  p.tiles = static_cast<uint32_t>(tiles);
+  p.status = ctx->d_status;
+  int rc = encode(ctx, &p.q, a.q, a.head, a.heads_q, a.rows_q, a.q_ld);
+  if (rc == B200_OK) rc = encode(ctx, &p.k, a.k, a.head, a.heads_k, a.rows_k, a.k_ld);
+  if (rc == B200_OK) rc = encode(ctx, &p.v, a.v, a.head, a.heads_k, a.rows_k, a.v_ld);
+  if (rc != B200_OK) return rc;
+  return a.head <= 64 ? launch_fw<64>(ctx, p, s) : launch_fw<128>(ctx, p, s);
+}
+
+}  // namespace b200
