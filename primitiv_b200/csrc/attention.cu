@@ -164,7 +164,7 @@ int b200_attention_bw(b200_ctx *ctx, int mode, const b200_attention *plan_host, 
   const u64 rows = static_cast<u64>(a.rows_q) * a.heads_q + static_cast<u64>(a.rows_k) * a.heads_k;
   B200_DISPATCH_MODE(mode, { b200::launch(ctx, attention_rows_kernel<T>, dim3(grid_for(ctx, rows, 8)), dim3(256), 0, s, 1u, a); });
   ++ctx->launches;
-  const int rc = attention_mma_bw(ctx, mode, a, s);
+  const int rc = attention_tc_bw_eligible(ctx, mode, a) ? attention_tc_bw(ctx, a, s) : attention_mma_bw(ctx, mode, a, s);
   if (rc != B200_OK) return rc;
   B200_OPS_EPILOGUE(ctx);
 }

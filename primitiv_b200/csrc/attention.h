@@ -35,6 +35,8 @@ int attention_mma_bw(b200_ctx *ctx, int mode, const AttnArgs &a, cudaStream_t s)
 // attention_tc.cu: halves on tcgen05
 bool attention_tc_fw_eligible(const b200_ctx *ctx, int mode, const AttnArgs &a);
 int attention_tc_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s);
+bool attention_tc_bw_eligible(const b200_ctx *ctx, int mode, const AttnArgs &a);
+int attention_tc_bw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s);
 
 #ifdef __CUDACC__
 

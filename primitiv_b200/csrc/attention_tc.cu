@@ -68,6 +68,13 @@ __device__ __forceinline__ void product_pn(uint32_t d, uint32_t p, uint32_t b, u
     mma_from_tmem(d, p + ks * 8, (((b + ks * 2048) & 0x3FFFFu) >> 4) | ((kChunk >> 4) << 16), kDescHi, idesc, !(first && ks == 0));
 }
 
+// The same with p in two runs of 32 columns, 64 apart: each half of the warps writes over its own half of s.
+__device__ __forceinline__ void product_pn2(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks)
+    mma_from_tmem(d, p + (ks >> 2) * 64 + (ks & 3) * 8, (((b + ks * 2048) & 0x3FFFFu) >> 4) | ((kChunk >> 4) << 16), kDescHi, idesc, !(first && ks == 0));
+}
+
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -97,6 +104,11 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   f32x2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint32_t halves_of(float lo, float hi) {
@@ -399,6 +411,390 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
   }
 }
 
+// ---- backward -----------------------------------------------------------------------------------------------
+//
+// Two kernels of one shape, as in attention_mma.cu, so that neither needs atomics: with 128 keys at rest (gk and gv; the queries of
+// all heads of the group pass by) and with 128 queries at rest (gq; the keys pass by).  X1, X2 rest, tiles Y1, Y2 come
+// through a ring:
+//   keys at rest     X1 = k, X2 = v, Y1 = q, Y2 = gy:   s' = k q^T, dp' = v gy^T,  gv += p' gy,  gk += ds' q
+//   queries at rest  X1 = q, X2 = gy, Y1 = k, Y2 = v:   s = q k^T,  dp = gy v^T,   gq += ds k
+// Transposed where the keys rest, so that p and ds are always the left operand, from tensor memory, where they take the place of s
+// and dp, and a tile in shared memory serves both as the right operand of the first products and of the second.  Eight
+// warps share a tile: a thread has 64 of a row's 128 columns.
+//   order of the products, keys at rest:     gv(i) s(i+1) gk(i) dp(i+1): p(i+1) is made beside the last two, ds(i+1) beside the first two
+//   queries at rest:                         s(i+1) gq(i) dp(i+1), with two buffers for s
+// Bound by the tensor core: 2048 + 1536 clocks per 128 x 128 pairs, against 1024 of the special function units in each.
+//
+// p and ds are halves.  p is stored as 2^13 p; ds after a scale by a power of two from the largest |ds| that the norms of gy and v
+// allow, over all that the block sees (keys at rest) or per query: without it the ds of long rows lie below the smallest half.
+
+struct alignas(64) BwParams {
+  CUtensorMap x1, x2, y1, y2;
+  AttnArgs a;
+  uint32_t tiles, columns;
+  int *status;
+};
+
+constexpr uint32_t kBwThreads = 384;
+template <int kD> constexpr uint32_t kBwStages = kD == 128 ? 2u : 4u;
+template <int kD> constexpr uint32_t kBwSmem = (2 + 2 * kBwStages<kD>) * kTile * kD * 2 + 1024;
+constexpr float kPBits = 13.f;
+
+// The power of two that takes the largest |ds| possible to at most 2^14.  |dp - delta| <= |gy| |v| + |delta|.
+__device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) {
+  const float bound = sqrtf(gy_sq) * sqrtf(v_sq) + delta;
+  if (!(bound > 1e-30f) || !(bound < 1e30f)) return 1.f;
+  return exp2f(fminf(fmaxf(13.f - ceilf(log2f(bound)), -100.f), 100.f));
+}
+
+template <int kD, bool kKeys>
+__global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __grid_constant__ BwParams p) {
+  constexpr uint32_t kBytes = kTile * kD * 2, kStages = kBwStages<kD>, kChunks = kD / 64;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t x_full, full_bar[kStages], ready_bar[kStages], empty_bar[kStages], s_full[2], dp_full, p_full, ds_full, acc_done, drain_bar;
+  __shared__ __align__(16) float s_stat[kKeys ? kStages : 1][2][kTile];   // -lse log2(e) + 13, and -delta, scaled
+  __shared__ float s_max[3][kBwThreads / 32];
+  __shared__ uint32_t tmem_slot, s_at[2];
+  __shared__ int s_abort;
+  pdl_release_next();
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem + 2 * kBytes;
+  volatile int *abort_flag = &s_abort;
+  const AttnArgs &a = p.a;
+  if (threadIdx.x == 9u * 32u) {
+    for (const CUtensorMap *m : {&p.x1, &p.x2, &p.y1, &p.y2}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(m)) : "memory");
+  }
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    mbar_init(smem_u32(&x_full), 1);
+    for (uint32_t i = 0; i < kStages; ++i)
+      mbar_init(smem_u32(&full_bar[i]), 1), mbar_init(smem_u32(&ready_bar[i]), 1), mbar_init(smem_u32(&empty_bar[i]), 1);
+    mbar_init(smem_u32(&s_full[0]), 1), mbar_init(smem_u32(&s_full[1]), 1), mbar_init(smem_u32(&dp_full), 1);
+    mbar_init(smem_u32(&p_full), 8), mbar_init(smem_u32(&ds_full), 8);
+    mbar_init(smem_u32(&acc_done), 1), mbar_init(smem_u32(&drain_bar), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait_previous();
+  tc_fence_before();
+  // heaviest first: the first keys of a causal sequence are seen by the most queries, its last queries see the most keys
+  const uint32_t column = blockIdx.x % p.columns, nth = blockIdx.x / p.columns;
+  uint32_t seq, tile;
+  const bool any = attn_find_tile<kKeys>(a, kKeys ? nth : p.tiles - 1u - nth, 1, kTile, s_at, seq, tile);
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  constexpr uint32_t kDp = kKeys ? kTile : 2 * kTile;                          // columns of dp
+  constexpr uint32_t kAcc1 = 2 * kTile, kAcc2 = kKeys ? 2 * kTile + kD : 3 * kTile;   // gv; gk or gq
+
+  if (any) {
+    const AttnSeq q = attn_seq(a, seq);
+    const long long shift = static_cast<long long>(q.lk) - q.lq;
+    const uint32_t kv_head = kKeys ? column : column / a.group, q_head = kKeys ? column * a.group : column;
+    const uint32_t row0 = tile * kTile, rows = kKeys ? q.lk : q.lq;
+    // what passes by: `per` tiles from `from` on, for each head of the group where those are queries
+    uint32_t from = 0, to = kKeys ? q.lq : q.lk;
+    if (a.causal) {
+      if (kKeys) {
+        const long long first = static_cast<long long>(row0) - shift;
+        from = first <= 0 ? 0u : (first >= q.lq ? q.lq : static_cast<uint32_t>(first));
+      } else {
+        const long long seen = static_cast<long long>(min(row0 + kTile, q.lq)) + shift;
+        to = seen <= 0 ? 0u : min(to, static_cast<uint32_t>(seen));
+      }
+    }
+    const uint32_t per = to > from ? (to - from + kTile - 1) / kTile : 0u, steps = kKeys ? per * a.group : per;
+    const uint32_t left = (to - from) % kTile;
+    const unsigned long long stat = static_cast<unsigned long long>(q_head) * a.rows_q + q.q0;
+
+    // the scale of ds
+    float gm = 0.f, dm = 0.f, vm = 0.f, ds_scale;
+    {
+      if constexpr (kKeys) {
+        for (uint32_t g = 0; g < a.group; ++g)
+#pragma unroll 4
+          for (uint32_t t = from + threadIdx.x; t < q.lq; t += kBwThreads) {
+            const unsigned long long i = stat + static_cast<unsigned long long>(g) * a.rows_q + t;
+            gm = fmaxf(gm, a.gy_norm[i]);
+            dm = fmaxf(dm, fabsf(a.delta[i]));
+          }
+      }
+      const uint32_t k_from = kKeys ? row0 : 0u, k_to = kKeys ? min(row0 + kTile, rows) : to;
+#pragma unroll 4
+      for (uint32_t t = k_from + threadIdx.x; t < k_to; t += kBwThreads)
+        vm = fmaxf(vm, a.v_norm[static_cast<unsigned long long>(kv_head) * a.rows_k + q.k0 + t]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+        dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, o));
+        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+      }
+      if (lane == 0) s_max[0][warp] = gm, s_max[1][warp] = dm, s_max[2][warp] = vm;
+      __syncthreads();
+#pragma unroll
+      for (uint32_t w = 0; w < kBwThreads / 32; ++w) gm = fmaxf(gm, s_max[0][w]), dm = fmaxf(dm, s_max[1][w]), vm = fmaxf(vm, s_max[2][w]);
+      ds_scale = scale_of(gm, vm, dm);
+    }
+
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 9) {
+      // ------------------------------ copies ------------------------------
+      if (steps > 0) {
+        uint32_t stage = 0, phase = 0, armed = 0, parity = 0;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(smem_u32(&x_full), 2 * kBytes);
+          for (uint32_t c = 0; c < kChunks; ++c) {
+            const int head = kKeys ? kv_head : q_head, row = (kKeys ? q.k0 : q.q0) + row0;
+            tma_load_3d(smem + c * kChunk, &p.x1, smem_u32(&x_full), c * 64, head, row);
+            tma_load_3d(smem + kBytes + c * kChunk, &p.x2, smem_u32(&x_full), c * 64, head, row);
+          }
+        }
+        __syncwarp();
+        uint32_t g = 0, t = 0;
+        for (uint32_t i = 0; i < steps; ++i) {
+          if (!wait_all(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) break;
+          const uint32_t bar = smem_u32(&full_bar[stage]), dst = ring + stage * 2 * kBytes;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar, 2 * kBytes);
+            const int head = kKeys ? q_head + g : kv_head, row = (kKeys ? q.q0 : q.k0) + from + t * kTile;
+            for (uint32_t c = 0; c < kChunks; ++c) {
+              tma_load_3d(dst + c * kChunk, &p.y1, bar, c * 64, head, row);
+              tma_load_3d(dst + kBytes + c * kChunk, &p.y2, bar, c * 64, head, row);
+            }
+          }
+          __syncwarp();
+          armed |= 1u << stage;
+          parity = (parity & ~(1u << stage)) | (phase << stage);
+          if (++t == per) t = 0, ++g;
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+        if (*abort_flag) {
+          mbar_wait_quiet(smem_u32(&x_full), 0);
+          for (uint32_t s = 0; s < kStages; ++s)
+            if (armed & (1u << s)) mbar_wait_quiet(smem_u32(&full_bar[s]), (parity >> s) & 1u);
+        }
+      }
+    } else if (warp == 10) {
+      // ------------------------------ what a tile needs before use: its rows' numbers, zeros behind its last row ------------------------------
+      uint32_t stage = 0, phase = 0, g = 0, t = 0;
+      for (uint32_t i = 0; i < steps; ++i) {
+        if (!wait_all(smem_u32(&full_bar[stage]), phase, abort_flag)) break;
+        if constexpr (kKeys) {
+          const float f = ds_scale * exp2f(-kPBits);
+#pragma unroll
+          for (uint32_t c = lane; c < kTile; c += 32u) {
+            const uint32_t tok = from + t * kTile + c;
+            const unsigned long long at = stat + static_cast<unsigned long long>(g) * a.rows_q + tok;
+            const float lse = tok < q.lq ? a.lse[at] : -INFINITY;
+            s_stat[stage][0][c] = lse == -INFINITY ? lse : kPBits - lse * kLog2e;
+            s_stat[stage][1][c] = tok < q.lq ? -a.delta[at] * f : 0.f;
+          }
+        }
+        if (t + 1 == per && left != 0u) {
+          const uint32_t base = ring + stage * 2 * kBytes;
+          for (uint32_t c = 0; c < 2 * kChunks; ++c)
+            for (uint32_t at = left * 128u + lane * 16u; at < kChunk; at += 512u)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + c * kChunk + at), "r"(0u) : "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ready_bar[stage]));
+        if (++t == per) t = 0, ++g;
+        if (++stage == kStages) stage = 0, phase ^= 1u;
+      }
+    } else if (warp == 8) {
+      // ------------------------------ products ------------------------------
+      if (steps > 0) {
+        constexpr uint32_t kS = idesc_of(kTile, 0), kG = idesc_of(kD, 1);
+        uint32_t stage = 0, phase = 0;
+        // (`ready` follows `full`, which is what orders the copies before the products)
+        auto tile_ready = [&](uint32_t s, uint32_t ph) { return wait_all(smem_u32(&ready_bar[s]), ph, abort_flag) && wait_all(smem_u32(&full_bar[s]), ph, abort_flag); };
+        bool ok = wait_all(smem_u32(&x_full), 0, abort_flag) && tile_ready(0, 0);
+        if (ok) {
+          product_nt<kD>(tmem, smem, ring, kS);
+          mma_commit(smem_u32(&s_full[0]));
+          product_nt<kD>(tmem + kDp, smem + kBytes, ring + kBytes, kS);
+          mma_commit(smem_u32(&dp_full));
+        }
+        for (uint32_t i = 0; ok && i < steps; ++i) {
+          const uint32_t y1 = ring + stage * 2 * kBytes, y2 = y1 + kBytes, this_stage = stage;
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+          const uint32_t next = ring + stage * 2 * kBytes;
+          const bool more = i + 1 < steps;
+          if constexpr (kKeys) {
+            if (!wait_all(smem_u32(&p_full), i & 1u, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            product_pn2(tmem + kAcc1, tmem, y2, kG, i == 0);
+          }
+          if (more) {
+            if (!tile_ready(stage, phase)) { ok = false; break; }
+            const uint32_t b = kKeys ? 0u : (i + 1) & 1u;
+            product_nt<kD>(tmem + b * kTile, smem, next, kS);
+            mma_commit(smem_u32(&s_full[b]));
+          }
+          if (!wait_all(smem_u32(&ds_full), i & 1u, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          product_pn2(tmem + kAcc2, tmem + kDp, y1, kG, i == 0);
+          mma_commit(smem_u32(&empty_bar[this_stage]));
+          if (more) {
+            product_nt<kD>(tmem + kDp, smem + kBytes, next + kBytes, kS);
+            mma_commit(smem_u32(&dp_full));
+          }
+        }
+        if (ok) mma_commit(smem_u32(&acc_done));
+        if (*abort_flag) {
+          __syncwarp();
+          mma_commit(smem_u32(&drain_bar));
+          mbar_wait_quiet(smem_u32(&drain_bar), 0);
+        }
+      }
+    } else if (warp < 8) {
+      // ------------------------------ p and ds ------------------------------
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+      const uint32_t half = warp >> 2, quarter = warp & 3u, col0 = half * 64u;
+      const uint32_t lanes = (quarter * 32u) << 16;
+      const uint32_t row = row0 + quarter * 32u + lane;
+      const float to2 = a.scale * kLog2e;
+      float base = 0.f, minus_delta = 0.f;
+      long long sees = q.lk;
+      if constexpr (!kKeys) {
+        if (row < rows) {
+          const float lse = a.lse[stat + row];
+          base = lse == -INFINITY ? 0.f : -lse * kLog2e;   // (a query that sees nothing: every column below is masked)
+          const float delta = a.delta[stat + row];
+          ds_scale = scale_of(a.gy_norm[stat + row], vm, fabsf(delta));
+          minus_delta = -delta * ds_scale;
+        }
+        if (a.causal) sees = min(sees, max(0ll, static_cast<long long>(row) + 1 + shift));
+      }
+      const float f = kKeys ? ds_scale * exp2f(-kPBits) : ds_scale;
+      const f32x2 to22 = pair_of(to2, to2), f2 = pair_of(f, f);
+      uint32_t stage = 0, phase = 0, t = 0;
+      bool ok = true;
+      for (uint32_t i = 0; i < steps; ++i) {
+        const uint32_t b = kKeys ? 0u : i & 1u, s_tmem = tmem + lanes + b * kTile + col0, dp_tmem = tmem + lanes + kDp + col0;
+        if (kKeys && !wait_all(smem_u32(&ready_bar[stage]), phase, abort_flag)) { ok = false; break; }
+        if (!wait_all(smem_u32(&s_full[b]), (kKeys ? i : i >> 1) & 1u, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t s[2][32];
+        tmem_ld32_issue(s_tmem, s[0]);
+        tmem_ld32_issue(s_tmem + 32, s[1]);
+        tmem_ld_wait(s[0]);
+        tmem_ld_wait(s[1]);
+        // columns of this thread that its row has no part in: [0, skip) where queries pass by, [skip, 64) where keys do
+        int skip;
+        if constexpr (kKeys) {
+          const long long first = a.causal ? static_cast<long long>(row) - shift - (from + static_cast<long long>(t) * kTile) - col0 : 0ll;
+          skip = static_cast<int>(max(0ll, min(first, 64ll)));
+        } else {
+          skip = static_cast<int>(max(0ll, min(sees - static_cast<long long>(i) * kTile - col0, 64ll)));
+        }
+        if (__any_sync(0xffffffffu, kKeys ? skip > 0 : skip < 64)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (kKeys ? c * 32 + e < skip : c * 32 + e >= skip) s[c][e] = 0xff800000u;
+        }
+        uint32_t out[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            f32x2 add = pair_of(base, base);
+            if constexpr (kKeys) add = *reinterpret_cast<const f32x2 *>(&s_stat[stage][0][col0 + c * 32 + e]);
+            float u, w;
+            unpair(fma2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), to22, add), u, w);
+            u = attn_exp2(u), w = attn_exp2(w);
+            s[c][e] = __float_as_uint(u), s[c][e + 1] = __float_as_uint(w);
+            if constexpr (kKeys) out[c * 16 + e / 2] = halves_of(u, w);
+          }
+        if constexpr (kKeys) {
+          tmem_st32(s_tmem, out);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&p_full));
+        }
+        if (!wait_all(smem_u32(&dp_full), i & 1u, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t d[2][32];
+        tmem_ld32_issue(dp_tmem, d[0]);
+        tmem_ld32_issue(dp_tmem + 32, d[1]);
+        tmem_ld_wait(d[0]);
+        tmem_ld_wait(d[1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            f32x2 add = pair_of(minus_delta, minus_delta);
+            if constexpr (kKeys) add = *reinterpret_cast<const f32x2 *>(&s_stat[stage][1][col0 + c * 32 + e]);
+            float u, w;
+            unpair(mul2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])),
+                        fma2(pair_of(__uint_as_float(d[c][e]), __uint_as_float(d[c][e + 1])), f2, add)), u, w);
+            out[c * 16 + e / 2] = halves_of(u, w);
+          }
+        tmem_st32(dp_tmem, out);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ds_full));
+        if (++t == per) t = 0;
+        if (++stage == kStages) stage = 0, phase ^= 1u;
+      }
+      if (ok && steps > 0) ok = wait_all(smem_u32(&acc_done), 0, abort_flag);
+      tc_fence_after();
+      if (ok) {
+        // keys at rest: gv by the first four warps, gk by the others; queries at rest: half of gq's columns each
+        const float undo = kKeys && half == 0 ? exp2f(-kPBits) : a.scale / ds_scale;
+        constexpr int kCols = kKeys ? kD : kD / 2;
+        const uint32_t c0 = kKeys ? 0u : half * kCols;
+        const uint32_t acc = tmem + lanes + (kKeys && half == 0 ? kAcc1 : kAcc2) + c0;
+        __half *out;
+        if constexpr (kKeys)
+          out = half == 0 ? static_cast<__half *>(a.gv) + (q.k0 + static_cast<unsigned long long>(row)) * a.v_ld + static_cast<unsigned long long>(kv_head) * a.head
+                          : static_cast<__half *>(a.gk) + (q.k0 + static_cast<unsigned long long>(row)) * a.k_ld + static_cast<unsigned long long>(kv_head) * a.head;
+        else
+          out = static_cast<__half *>(a.gq) + (q.q0 + static_cast<unsigned long long>(row)) * a.q_ld + static_cast<unsigned long long>(q_head) * a.head;
+#pragma unroll
+        for (int c = 0; c < kCols; c += 32) {
+          uint32_t y[32];
+          if (steps > 0) tmem_ld32(acc + c, y);
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (row < rows && c0 + c + e < a.head) {
+              float v[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[k] = steps > 0 ? __uint_as_float(y[e + k]) * undo : 0.f;
+              uint4 *to16 = reinterpret_cast<uint4 *>(out + c0 + c + e);
+              if (a.accumulate) {
+                const uint4 old = *to16;
+                const uint32_t words[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&words[k]));
+                  v[2 * k] += o.x, v[2 * k + 1] += o.y;
+                }
+              }
+              *to16 = make_uint4(halves_of(v[0], v[1]), halves_of(v[2], v[3]), halves_of(v[4], v[5]), halves_of(v[6], v[7]));
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && s_abort) report_status(p.status, B200_ERR_KERNEL_TIMEOUT);
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 // ---- launches ------------------------------------------------------------------------------------------------
 
 // Shape({head, heads, rows}) in boxes of 64 elements of one head of 128 rows; what lies past the head or the rows reads as zero.
@@ -419,6 +815,17 @@ int launch_fw(b200_ctx *ctx, const FwParams &p, cudaStream_t s) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kFwSmem<kD>));
   if (e != cudaSuccess) return static_cast<int>(e);
   b200::launch(ctx, kernel, dim3(p.tiles * p.columns), dim3(kFwThreads), kFwSmem<kD>, s, 1u, p);
+  return B200_OK;
+}
+
+template <int kD, bool kKeys>
+int launch_bw(b200_ctx *ctx, const BwParams &p, cudaStream_t s) {
+  if (p.tiles == 0) return B200_OK;
+  auto kernel = attention_bw_tc_kernel<kD, kKeys>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBwSmem<kD>));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  b200::launch(ctx, kernel, dim3(p.tiles * p.columns), dim3(kBwThreads), kBwSmem<kD>, s, 1u, p);
+  ++ctx->launches;
   return B200_OK;
 }
 
@@ -444,6 +851,33 @@ int attention_tc_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
   if (rc == B200_OK) rc = encode(ctx, &p.v, a.v, a.head, a.heads_k, a.rows_k, a.v_ld);
   if (rc != B200_OK) return rc;
   return a.head <= 64 ? launch_fw<64>(ctx, p, s) : launch_fw<128>(ctx, p, s);
+}
+
+bool attention_tc_bw_eligible(const b200_ctx *ctx, int mode, const AttnArgs &a) {
+  return mode == B200_MODE_FP16 && ctx->encode_tiled && a.head <= 128 && a.head % 8 == 0 && a.max_k > 0 && a.max_q > 0 && a.seqs > 0 &&
+         addressable(a.q, a.q_ld) && addressable(a.k, a.k_ld) && addressable(a.v, a.v_ld) && addressable(a.gy, a.y_ld) &&
+         addressable(a.gq, a.q_ld) && addressable(a.gk, a.k_ld) && addressable(a.gv, a.v_ld) && a.scale > 0.f;
+}
+
+int attention_tc_bw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
+  CUtensorMap q, k, v, gy;
+  int rc = encode(ctx, &q, a.q, a.head, a.heads_q, a.rows_q, a.q_ld);
+  if (rc == B200_OK) rc = encode(ctx, &k, a.k, a.head, a.heads_k, a.rows_k, a.k_ld);
+  if (rc == B200_OK) rc = encode(ctx, &v, a.v, a.head, a.heads_k, a.rows_k, a.v_ld);
+  if (rc == B200_OK) rc = encode(ctx, &gy, a.gy, a.head, a.heads_q, a.rows_q, a.y_ld);
+  if (rc != B200_OK) return rc;
+  const unsigned long long k_tiles = attn_tile_bound(a.rows_k, a.max_k, a.seqs, 1, kTile), q_tiles = attn_tile_bound(a.rows_q, a.max_q, a.seqs, 1, kTile);
+  if (k_tiles * a.heads_k > 0x7fffffffull || q_tiles * a.heads_q > 0x7fffffffull) return B200_ERR_TOO_LARGE;
+  BwParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.a = a, p.status = ctx->d_status;
+  p.x1 = k, p.x2 = v, p.y1 = q, p.y2 = gy, p.tiles = static_cast<uint32_t>(k_tiles), p.columns = a.heads_k;
+  rc = a.head <= 64 ? launch_bw<64, true>(ctx, p, s) : launch_bw<128, true>(ctx, p, s);
+  if (rc != B200_OK) return rc;
+  p.x1 = q, p.x2 = gy, p.y1 = k, p.y2 = v, p.tiles = static_cast<uint32_t>(q_tiles), p.columns = a.heads_q;
+  rc = a.head <= 64 ? launch_bw<64, false>(ctx, p, s) : launch_bw<128, false>(ctx, p, s);
+  --ctx->launches;   // the entry point counts the last one
+  return rc;
 }
 
 }  // namespace b200
