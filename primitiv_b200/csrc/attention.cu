@@ -139,8 +139,10 @@ int b200_attention_fw(b200_ctx *ctx, int mode, const b200_attention *plan_host, 
   if (!q || !y || (a.rows_k > 0 && (!k || !v))) return B200_ERR_INVALID_ARG;
   a.q = q, a.k = k, a.v = v, a.y = y, a.lse = lse;
   ProfScope prof(ctx, kProfElementwise, s);
-  const bool tc = a.max_q > 64 && attention_tc_fw_eligible(ctx, mode, a);
-  const int rc = tc ? attention_tc_fw(ctx, a, s) : attention_mma_fw(ctx, mode, a, s);
+  int rc;
+  if (static_cast<u64>(a.max_q) * a.group <= 32u && a.max_k > 0) rc = attention_tokens_fw(ctx, mode, a, s);
+  else if (a.max_q > 64 && attention_tc_fw_eligible(ctx, mode, a)) rc = attention_tc_fw(ctx, a, s);
+  else rc = attention_mma_fw(ctx, mode, a, s);
   if (rc != B200_OK) return rc;
   B200_OPS_EPILOGUE(ctx);
 }

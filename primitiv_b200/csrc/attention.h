@@ -32,6 +32,8 @@ struct AttnArgs {
 int attention_mma_fw(b200_ctx *ctx, int mode, const AttnArgs &a, cudaStream_t s);
 int attention_mma_bw(b200_ctx *ctx, int mode, const AttnArgs &a, cudaStream_t s);
 
+// attention_tokens.cu: a few queries per sequence
+int attention_tokens_fw(b200_ctx *ctx, int mode, const AttnArgs &a, cudaStream_t s);
 // attention_tc.cu: halves on tcgen05
 bool attention_tc_fw_eligible(const b200_ctx *ctx, int mode, const AttnArgs &a);
 int attention_tc_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s);
