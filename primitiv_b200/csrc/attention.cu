@@ -29,60 +29,78 @@ __device__ __forceinline__ bool in_sequence(const uint32_t *starts, const uint32
   return t >= first && t - first < len;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Eight elements of a head's row from d on, zeros past `head`; one 16- or 32-byte piece where `wide`.
+template <typename T>
+__device__ __forceinline__ void load8(float (&v)[8], const T *p, uint32_t d, uint32_t head, bool wide) {
+  if (wide) {
+    constexpr int N = Vec<T>::N;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+    for (int i = 0; i < 8; i += N) {
+      Vec<T> x;
+      if (d + i < head) x.load(p + d + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i + j] = d + i < head ? x.get(j) : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = d + i < head ? ld(p, d + i) : 0.f;
+  }
 }
 
-// delta[h][t] = sum_d gy y, and the squares' sums that the kernels for halves take their scales from; one warp a head
-// of a row.  Gradients of rows outside every sequence, which no other kernel touches, are stored as zeros here.
+// delta[h][t] = sum_d gy y, and the squares' sums that the kernels for halves take their scales from.  Gradients of rows
+// outside every sequence, which no other kernel touches, are stored as zeros here.  A warp takes a row; a group of lanes (the least
+// power of two that holds a head at eight elements a lane) takes a head.  Bound by memory: y, gy and v once.
 template <typename T>
-__global__ void __launch_bounds__(256) attention_rows_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256) attention_rows_kernel(AttnArgs a, uint32_t lanes, int wide) {
   pdl_enter();
-  const uint32_t lane = threadIdx.x & 31u;
-  const u64 nq = static_cast<u64>(a.rows_q) * a.heads_q, nk = static_cast<u64>(a.rows_k) * a.heads_k;
-  for (u64 w = static_cast<u64>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < nq + nk; w += static_cast<u64>(gridDim.x) * 8) {
-    if (w < nq) {
-      const uint32_t t = static_cast<uint32_t>(w / a.heads_q), h = static_cast<uint32_t>(w - static_cast<u64>(t) * a.heads_q);
+  const uint32_t lane = threadIdx.x & 31u, at = lane & (lanes - 1), group = lane / lanes, groups = 32u / lanes, d = at * 8u;
+  const u64 rows = static_cast<u64>(a.rows_q) + a.rows_k;
+  for (u64 w = static_cast<u64>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < rows; w += static_cast<u64>(gridDim.x) * 8) {
+    if (w < a.rows_q) {
+      const uint32_t t = static_cast<uint32_t>(w);
       if (!in_sequence(a.q_starts, a.q_lens, a.q_pitch, a.rows_q, a.max_q, a.seqs, t)) {
         if (!a.accumulate)
-          for (uint32_t d = lane; d < a.head; d += 32) st(static_cast<T *>(a.gq), t * a.q_ld + static_cast<u64>(h) * a.head + d, 0.f);
+          for (uint32_t i = lane; i < a.heads_q * a.head; i += 32) st(static_cast<T *>(a.gq), t * a.q_ld + i, 0.f);
         continue;
       }
-      const T *gy = static_cast<const T *>(a.gy) + t * a.y_ld + static_cast<u64>(h) * a.head;
-      const T *y = static_cast<const T *>(a.y_in) + t * a.y_ld + static_cast<u64>(h) * a.head;
-      float dot = 0.f, sq = 0.f;
-      for (uint32_t d = lane; d < a.head; d += 32) {
-        const float g = ld(gy, d);
-        dot += g * ld(y, d);
-        sq += g * g;
-      }
-      dot = warp_sum(dot);
-      sq = warp_sum(sq);
-      if (lane == 0) {
-        a.delta[static_cast<u64>(h) * a.rows_q + t] = dot;
-        a.gy_norm[static_cast<u64>(h) * a.rows_q + t] = sq;
+      const T *gy = static_cast<const T *>(a.gy) + t * a.y_ld, *y = static_cast<const T *>(a.y_in) + t * a.y_ld;
+#pragma unroll 2
+      for (uint32_t h0 = 0; h0 < a.heads_q; h0 += groups) {
+        const uint32_t h = h0 + group;
+        float g[8], v[8], dot = 0.f, sq = 0.f;
+        load8(g, gy + static_cast<u64>(h) * a.head, h < a.heads_q ? d : a.head, a.head, wide);
+        load8(v, y + static_cast<u64>(h) * a.head, h < a.heads_q ? d : a.head, a.head, wide);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot += g[i] * v[i], sq += g[i] * g[i];
+        for (uint32_t o = 1; o < lanes; o <<= 1) {
+          dot += __shfl_xor_sync(0xffffffffu, dot, o);
+          sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        }
+        if (at == 0 && h < a.heads_q) {
+          a.delta[static_cast<u64>(h) * a.rows_q + t] = dot;
+          a.gy_norm[static_cast<u64>(h) * a.rows_q + t] = sq;
+        }
       }
     } else {
-      const u64 wk = w - nq;
-      const uint32_t t = static_cast<uint32_t>(wk / a.heads_k), h = static_cast<uint32_t>(wk - static_cast<u64>(t) * a.heads_k);
+      const uint32_t t = static_cast<uint32_t>(w - a.rows_q);
       if (!in_sequence(a.k_starts, a.k_lens, a.k_pitch, a.rows_k, a.max_k, a.seqs, t)) {
         if (!a.accumulate)
-          for (uint32_t d = lane; d < a.head; d += 32) {
-            st(static_cast<T *>(a.gk), t * a.k_ld + static_cast<u64>(h) * a.head + d, 0.f);
-            st(static_cast<T *>(a.gv), t * a.v_ld + static_cast<u64>(h) * a.head + d, 0.f);
+          for (uint32_t i = lane; i < a.heads_k * a.head; i += 32) {
+            st(static_cast<T *>(a.gk), t * a.k_ld + i, 0.f);
+            st(static_cast<T *>(a.gv), t * a.v_ld + i, 0.f);
           }
         continue;
       }
-      const T *v = static_cast<const T *>(a.v) + t * a.v_ld + static_cast<u64>(h) * a.head;
-      float sq = 0.f;
-      for (uint32_t d = lane; d < a.head; d += 32) {
-        const float x = ld(v, d);
-        sq += x * x;
+      const T *v = static_cast<const T *>(a.v) + t * a.v_ld;
+      for (uint32_t h0 = 0; h0 < a.heads_k; h0 += groups) {
+        const uint32_t h = h0 + group;
+        float x[8], sq = 0.f;
+        load8(x, v + static_cast<u64>(h) * a.head, h < a.heads_k ? d : a.head, a.head, wide);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
+        for (uint32_t o = 1; o < lanes; o <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        if (at == 0 && h < a.heads_k) a.v_norm[static_cast<u64>(h) * a.rows_k + t] = sq;
       }
-      sq = warp_sum(sq);
-      if (lane == 0) a.v_norm[static_cast<u64>(h) * a.rows_k + t] = sq;
     }
   }
 }
@@ -163,8 +181,13 @@ int b200_attention_bw(b200_ctx *ctx, int mode, const b200_attention *plan_host, 
   a.gy_norm = a.delta + static_cast<u64>(a.rows_q) * a.heads_q;
   a.v_norm = a.gy_norm + static_cast<u64>(a.rows_q) * a.heads_q;
   ProfScope prof(ctx, kProfElementwise, s);
-  const u64 rows = static_cast<u64>(a.rows_q) * a.heads_q + static_cast<u64>(a.rows_k) * a.heads_k;
-  B200_DISPATCH_MODE(mode, { b200::launch(ctx, attention_rows_kernel<T>, dim3(grid_for(ctx, rows, 8)), dim3(256), 0, s, 1u, a); });
+  uint32_t lanes = 1;
+  while (lanes * 8 < a.head) lanes *= 2;
+  const u64 es = elem_bytes(mode);
+  const bool wide = aligned16(gy) && aligned16(y) && aligned16(v) && a.y_ld * es % 16 == 0 && a.v_ld * es % 16 == 0 && a.head * es % 16 == 0;
+  B200_DISPATCH_MODE(mode, {
+    b200::launch(ctx, attention_rows_kernel<T>, dim3(grid_for(ctx, static_cast<u64>(a.rows_q) + a.rows_k, 8)), dim3(256), 0, s, 1u, a, lanes, wide);
+  });
   ++ctx->launches;
   const int rc = attention_tc_bw_eligible(ctx, mode, a) ? attention_tc_bw(ctx, a, s) : attention_mma_bw(ctx, mode, a, s);
   if (rc != B200_OK) return rc;

@@ -1,13 +1,17 @@
 // Attention of halves on the tcgen05 tensor cores, for heads of up to 128 elements that TMA can address.
 //
 // Forward.  A block has two tiles of 128 queries that share their keys: two heads of one group where the group is
-// even, else 256 queries of one head.  Warps 0-3 and 4-7 are the softmax of one tile each, a thread a row; warp 8
-// issues every matrix instruction, warp 9 every copy.  Keys and values come through one ring of 128-row tiles.
+// even, else 256 queries of one head.  Warp 0 issues every matrix instruction, warp 1 every copy; warps 4-7 and
+// 8-11 are the softmax of one tile each, a thread a row.  Keys and values come through a ring each.
 //   tensor memory: s of tile 0, s of tile 1 (128 columns each), y of tile 0, y of tile 1
-//   p is written over s as halves, and is the left operand of p v from there: it never passes through shared memory
-// While one tile's rows are in their softmax, the tensor core has the other tile's two products: per 128 keys of one tile
-// 1024 clocks of matrix instructions stand against 16384 exponentials, which are 1024 clocks of the special function
-// units.  The products run in the order in which they were issued, so p(j) v is read before s(j + 1) overwrites it.
+// p is written over s as halves, and is the left operand of p v from there: it never passes through shared memory.  While one
+// tile's rows are in their softmax, the tensor core has the other tile's two products: per 128 keys of one tile 1024 clocks of
+// matrix instructions stand against 16384 exponentials, which are 1024 clocks of the special function units.  The products run
+// in the order in which they were issued, so p(j) v is read before s(j + 1) overwrites it.
+// 16384 causal tokens of 32 heads of 128 on 8: 1.82 ms, 1.21 PFLOP/s, at about 1.6 GHz and the GPU's 1000 W; 60 % of the tensor core's clocks.
+// What is left is the way round: a softmax of 1700 clocks, two products, 600 clocks of waking one another.  Tried and no better: one place
+// for s, which the tiles have in turn, p beside it (1.83 ms); the same with pairs of blocks that share each tile of keys and
+// values, so that the tensor core reads less of shared memory (2.03 ms).
 //
 // The running maximum that scales y is only moved when a row has passed it by more than 2^8: until then p may exceed one (at most
 // 256, exact enough in halves), and y stays in tensor memory untouched.  Moving it costs a pass over y, by the softmax
@@ -31,48 +35,58 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // ---- matrix instructions ------------------------------------------------------------------------------------
 
-// Left operand from tensor memory.  All lanes of a converged warp, uniform arguments.
-__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p, e;\n\t"
-      ".reg .b64 db;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t"
-      "}\n" ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
+// The instruction cache is what these warps wait for most: their code runs once per tile between two others that are unrolled over a
+// row, and each line of it comes from afar (a wait that had nothing to wait for took 300 clocks, loop and bookkeeping as
+// much again).  So a product is one run of eight instructions with little between them, waits keep their rare part elsewhere, and
+// one lane is elected once.
 // fp32 accumulator, both operands halves, M = 128, N columns; `mn`: the right operand lies N-major (its rows are k).
 constexpr uint32_t idesc_of(uint32_t n, uint32_t mn) { return (1u << 4) | (mn << 16) | ((n >> 3) << 17) | ((kTile >> 4) << 24); }
 // 128-byte swizzle, groups of eight lines 1024 bytes apart
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 
-// d[128][128 or N] = A . B^T over kD columns, both tiles of 128-byte lines in chunks of 64 columns.
-template <int kD>
-__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
-#pragma unroll
-  for (int c = 0; c < kD / 64; ++c)
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const uint32_t at = c * kChunk + ks * 32;
-      mma_issue<1, true>(d, ((a + at) & 0x3FFFFu) >> 4, kDescHi, ((b + at) & 0x3FFFFu) >> 4, kDescHi, idesc, (c | ks) != 0);
-    }
-}
-// d[128][kD] (+)= P . B, P of 128 halves a row in tensor memory, B a tile of 128 rows.
-__device__ __forceinline__ void product_pn(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first) {
-#pragma unroll
-  for (int ks = 0; ks < 8; ++ks)
-    mma_from_tmem(d, p + ks * 8, (((b + ks * 2048) & 0x3FFFFu) >> 4) | ((kChunk >> 4) << 16), kDescHi, idesc, !(first && ks == 0));
-}
 
-// The same with p in two runs of 32 columns, 64 apart: each half of the warps writes over its own half of s.
-__device__ __forceinline__ void product_pn2(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first) {
-#pragma unroll
-  for (int ks = 0; ks < 8; ++ks)
-    mma_from_tmem(d, p + (ks >> 2) * 64 + (ks & 3) * 8, (((b + ks * 2048) & 0x3FFFFu) >> 4) | ((kChunk >> 4) << 16), kDescHi, idesc, !(first && ks == 0));
+#define B200_MMA_SS "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, "
+#define B200_MMA_TS "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %4, "
+#define B200_NEXT_SS "add.u64 da, da, 2; add.u64 db, db, 2;\n\t"
+#define B200_NEXT_TS(COLUMNS) "add.u32 a, a, " COLUMNS "; add.u64 db, db, 128;\n\t"
+
+// d[128][128] = A . B^T over kD columns, both tiles of 128-byte lines in chunks of 64 columns.  All lanes of a converged warp, uniform
+// arguments; `leader`: not 0 in the one lane that issues.
+#define B200_NT_HEAD \
+  "{\n\t.reg .pred e, t, f;\n\t.reg .b64 da, db;\n\t" \
+  "setp.ne.b32 e, %5, 0; setp.eq.b32 t, %3, %3; setp.ne.b32 f, %3, %3;\n\tmov.b64 da, {%1, %3}; mov.b64 db, {%2, %3};\n\t"
+#define B200_NT_FOUR(FIRST) \
+  B200_MMA_SS FIRST ";\n\t" B200_NEXT_SS B200_MMA_SS "t;\n\t" B200_NEXT_SS B200_MMA_SS "t;\n\t" B200_NEXT_SS B200_MMA_SS "t;\n\t"
+#define B200_NT_ARGS ::"r"(d), "r"((a & 0x3FFFFu) >> 4), "r"((b & 0x3FFFFu) >> 4), "r"(kDescHi), "r"(idesc), "r"(leader) : "memory"
+template <int kD>
+__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t leader) {
+  static_assert(kChunk / 16 - 6 == 1018, "the step from the last of a chunk to the first of the next");
+  if constexpr (kD == 64) asm volatile(B200_NT_HEAD B200_NT_FOUR("f") "}\n" B200_NT_ARGS);
+  else asm volatile(B200_NT_HEAD B200_NT_FOUR("f") "add.u64 da, da, 1018; add.u64 db, db, 1018;\n\t" B200_NT_FOUR("t") "}\n" B200_NT_ARGS);
+}
+// d[128][N] (+)= P . B, P of 128 halves a row in tensor memory, B a tile of 128 rows in chunks of 64 columns.  kGap: p lies in two runs of
+// 32 columns, 64 apart.
+#define B200_PN(MIDDLE) \
+  "{\n\t.reg .pred e, t, f;\n\t.reg .b32 a;\n\t.reg .b64 db;\n\t" \
+  "setp.ne.b32 e, %5, 0; setp.eq.b32 t, %3, %3; setp.ne.b32 f, %6, 0;\n\tmov.b32 a, %1; mov.b64 db, {%2, %3};\n\t" \
+  B200_MMA_TS "f;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" \
+  B200_NEXT_TS(MIDDLE) B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") \
+  B200_MMA_TS "t;\n\t}\n"
+#define B200_PN_ARGS \
+  ::"r"(d), "r"(p), "r"(((b & 0x3FFFFu) >> 4) | ((kChunk >> 4) << 16)), "r"(kDescHi), "r"(idesc), "r"(leader), "r"(first ? 0u : 1u) : "memory"
+template <bool kGap = false>
+__device__ __forceinline__ void product_pn(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first, uint32_t leader) {
+  if constexpr (kGap) asm volatile(B200_PN("40") B200_PN_ARGS);
+  else asm volatile(B200_PN("8") B200_PN_ARGS);
+}
+// Arrives on `bar` when every product issued so far is done.
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t leader) {
+  asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar), "r"(leader) : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}\n" : "=r"(is));
+  return is;
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -117,8 +131,50 @@ __device__ __forceinline__ uint32_t halves_of(float lo, float hi) {
   return r;
 }
 
+// The larger one, or a NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x without the special function unit: x = n + r, |r| <= 1/2, n by adding and taking away 1.5 2^23, whose last bits it then is; 2^r by a
+// polynomial of degree 4 fitted for the least relative error (2.7e-6, a hundredth of what rounding to a half
+// costs); 2^n is n in an exponent's place.  Below 2^-126: next to nothing, as it should be.  A NaN stays one.
+__device__ __forceinline__ void exp2_by_products(f32x2 x, float &u, float &w) {
+  constexpr float kMagic = 12582912.f;
+  unpair(x, u, w);
+  x = pair_of(max_nan(u, -126.f), max_nan(w, -126.f));
+  const f32x2 t = add2(x, pair_of(kMagic, kMagic)), r = fma2(add2(t, pair_of(-kMagic, -kMagic)), pair_of(-1.f, -1.f), x);
+  f32x2 y = fma2(r, pair_of(0.009570102f, 0.009570102f), pair_of(0.055917863f, 0.055917863f));
+  y = fma2(y, r, pair_of(0.240247443f, 0.240247443f));
+  y = fma2(y, r, pair_of(0.693121791f, 0.693121791f));
+  y = fma2(y, r, pair_of(0.999999285f, 0.999999285f));
+  unpair(t, u, w);
+  unpair(mul2(y, pair_of(__uint_as_float((__float_as_uint(u) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(w) << 23) + 0x3f800000u))), u, w);
+}
+// Of eight pairs, kByProducts go that way: the special function units of an SM do 16 elements a clock, as many as its tensor core needs of
+// them at full rate.  More of them cost more instructions than they save: a warp is alone on its scheduler for most of its softmax.
+// (0, 1, 2, 3 of 8: 1.84, 1.82, 1.86, 1.88 ms for the 16384 tokens above.)
+constexpr int kByProducts = 1;
+__device__ __forceinline__ void exp2_pair(int nth, f32x2 x, float &u, float &w) {
+  if ((nth & 7) < kByProducts) {
+    exp2_by_products(x, u, w);
+  } else {
+    unpair(x, u, w);
+    u = attn_exp2(u), w = attn_exp2(w);
+  }
+}
+
 // All lanes of the warp.
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
@@ -132,36 +188,38 @@ struct alignas(64) FwParams {
   int *status;
 };
 
-constexpr uint32_t kFwThreads = 384;   // three warps on each quarter of an SM; the last two only lend their registers
-
-template <int kD> constexpr uint32_t kFwStages = kD == 128 ? 5u : 8u;
-template <int kD> constexpr uint32_t kFwSmem = (2 + kFwStages<kD>) * kTile * kD * 2 + 1024;
+constexpr uint32_t kFwThreads = 384;   // three warps on each quarter of an SM; two of the first four only lend their registers
+// Slots for tiles of keys and of values.
+template <int kD> constexpr uint32_t kFwK = kD == 128 ? 2u : 4u;
+template <int kD> constexpr uint32_t kFwV = kD == 128 ? 3u : 4u;
+template <int kD> constexpr uint32_t kFwSmem = (2 + kFwK<kD> + kFwV<kD>) * kTile * kD * 2 + 1024;
 
 template <int kD>
 __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __grid_constant__ FwParams p) {
-  constexpr uint32_t kBytes = kTile * kD * 2, kStages = kFwStages<kD>, kChunks = kD / 64;
+  constexpr uint32_t kBytes = kTile * kD * 2, kSlotsK = kFwK<kD>, kSlotsV = kFwV<kD>, kChunks = kD / 64;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full, full_bar[kStages], empty_bar[kStages], s_full[2], p_full[2], y_done[2], v_clean, drain_bar;
+  __shared__ __align__(8) uint64_t q_full, k_full[kSlotsK], k_empty[kSlotsK], v_full[kSlotsV], v_empty[kSlotsV], s_full[2], p_full[2], y_done[2], v_clean, drain_bar;
   __shared__ uint32_t tmem_slot, s_at[2];
   __shared__ int s_abort;
   pdl_release_next();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem + 2 * kBytes;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, k_ring = smem + 2 * kBytes, v_ring = k_ring + kSlotsK * kBytes;
   volatile int *abort_flag = &s_abort;
   const AttnArgs &a = p.a;
-  if (threadIdx.x == 9u * 32u) {
+  if (threadIdx.x == 32u) {
     for (const CUtensorMap *m : {&p.q, &p.k, &p.v}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(m)) : "memory");
   }
   if (threadIdx.x == 0) {
     s_abort = 0;
     mbar_init(smem_u32(&q_full), 1);
-    for (uint32_t i = 0; i < kStages; ++i) mbar_init(smem_u32(&full_bar[i]), 1), mbar_init(smem_u32(&empty_bar[i]), 1);
+    for (uint32_t i = 0; i < kSlotsK; ++i) mbar_init(smem_u32(&k_full[i]), 1), mbar_init(smem_u32(&k_empty[i]), 1);
+    for (uint32_t i = 0; i < kSlotsV; ++i) mbar_init(smem_u32(&v_full[i]), 1), mbar_init(smem_u32(&v_empty[i]), 1);
     for (uint32_t x = 0; x < 2; ++x) mbar_init(smem_u32(&s_full[x]), 1), mbar_init(smem_u32(&p_full[x]), 4), mbar_init(smem_u32(&y_done[x]), 1);
     mbar_init(smem_u32(&v_clean), 1);
     mbar_init(smem_u32(&drain_bar), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -177,58 +235,50 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
   if (any) {
     const AttnSeq q = attn_seq(a, seq);
     const long long shift = static_cast<long long>(q.lk) - q.lq;
-    const uint32_t head0 = p.two_heads ? 2 * column : column, kv_head = head0 / a.group;
-    uint32_t tok0[2], tiles[2], keys = 0, steps = 0;
-    bool has[2];
-#pragma unroll
-    for (uint32_t x = 0; x < 2; ++x) {
-      tok0[x] = tile * unit + (p.two_heads ? 0u : x * kTile);
-      has[x] = tok0[x] < q.lq;
-      uint32_t n = q.lk;
-      if (a.causal) {
-        const long long seen = static_cast<long long>(min(tok0[x] + kTile, q.lq)) + shift;
-        n = seen <= 0 ? 0u : min(n, static_cast<uint32_t>(seen));
-      }
-      tiles[x] = has[x] ? (n + kTile - 1) / kTile : 0u;
-      if (has[x]) keys = max(keys, n);
-      steps = max(steps, tiles[x]);
+    const uint32_t head0 = p.two_heads ? 2 * column : column, kv_head = head0 / a.group, first_tok = tile * unit;
+    auto head_of = [&](uint32_t x) { return head0 + (p.two_heads ? x : 0u); };
+    auto tok_of = [&](uint32_t x) { return first_tok + (p.two_heads ? 0u : x * kTile); };
+    // the keys that any of them sees: of two tiles of one head the first sees fewer, and has its last steps masked
+    uint32_t keys = q.lk;
+    if (a.causal) {
+      const long long seen = static_cast<long long>(min(first_tok + unit, q.lq)) + shift;
+      keys = seen <= 0 ? 0u : min(keys, static_cast<uint32_t>(seen));
     }
+    const uint32_t steps = (keys + kTile - 1) / kTile, count = p.two_heads || first_tok + kTile < q.lq ? 2u : 1u;
     const uint32_t left = keys % kTile;   // keys in the last tile, 0 = all
 
     // 168 registers a thread at launch: 56 + 2 * 224 = 3 * 168
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 9) {
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 1) {
       // ------------------------------ copies ------------------------------
       if (steps > 0) {
-        uint32_t stage = 0, phase = 0, armed = 0, parity = 0;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(smem_u32(&q_full), ((has[0] ? 1u : 0u) + (has[1] ? 1u : 0u)) * kBytes);
-          for (uint32_t x = 0; x < 2; ++x)
-            for (uint32_t c = 0; c < kChunks; ++c)
-              if (has[x]) tma_load_3d(smem + x * kBytes + c * kChunk, &p.q, smem_u32(&q_full), c * 64, head0 + (p.two_heads ? x : 0u), q.q0 + tok0[x]);
-        }
-        __syncwarp();
-        bool ok = true;
-        uint32_t last_bar = 0, last_parity = 0, last_at = 0;
-        for (uint32_t i = 0; ok && i < 2 * steps; ++i) {   // keys, values, keys, values, ...
-          if (!wait_all(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const uint32_t bar = smem_u32(&full_bar[stage]), dst = ring + stage * kBytes;
+        auto copy = [&](const CUtensorMap *map, uint32_t full, uint32_t dst, uint32_t j) {
           if (lane == 0) {
-            mbar_arrive_expect_tx(bar, kBytes);
-            for (uint32_t c = 0; c < kChunks; ++c) tma_load_3d(dst + c * kChunk, (i & 1u) ? &p.v : &p.k, bar, c * 64, kv_head, q.k0 + (i >> 1) * kTile);
+            mbar_arrive_expect_tx(full, kBytes);
+            for (uint32_t c = 0; c < kChunks; ++c) tma_load_3d(dst + c * kChunk, map, full, c * 64, kv_head, q.k0 + j * kTile);
           }
           __syncwarp();
-          armed |= 1u << stage;
-          parity = (parity & ~(1u << stage)) | (phase << stage);
-          last_bar = bar, last_parity = phase, last_at = dst;
-          if (++stage == kStages) stage = 0, phase ^= 1u;
+        };
+        if (lane == 0) {
+          mbar_arrive_expect_tx(smem_u32(&q_full), count * kBytes);
+          for (uint32_t x = 0; x < count; ++x)
+            for (uint32_t c = 0; c < kChunks; ++c) tma_load_3d(smem + x * kBytes + c * kChunk, &p.q, smem_u32(&q_full), c * 64, head_of(x), q.q0 + tok_of(x));
+        }
+        __syncwarp();
+        uint32_t copied_k = 0, copied_v = 0;
+        for (uint32_t j = 0; j < steps; ++j) {
+          const uint32_t ks = j % kSlotsK, vs = j % kSlotsV;
+          if (!wait_all(smem_u32(&k_empty[ks]), (j / kSlotsK & 1u) ^ 1u, abort_flag)) break;
+          copy(&p.k, smem_u32(&k_full[ks]), k_ring + ks * kBytes, j);
+          copied_k = j + 1;
+          if (!wait_all(smem_u32(&v_empty[vs]), (j / kSlotsV & 1u) ^ 1u, abort_flag)) break;
+          copy(&p.v, smem_u32(&v_full[vs]), v_ring + vs * kBytes, j);
+          copied_v = j + 1;
         }
         // The last tile of values: rows behind the last key hold another sequence's, or anything; p is zero there, but zero
         // times an infinity is not.
-        if (ok && left != 0u && wait_all(last_bar, last_parity, abort_flag)) {
+        const uint32_t end = steps - 1u, last_at = v_ring + end % kSlotsV * kBytes;
+        if (copied_v == steps && left != 0u && wait_all(smem_u32(&v_full[end % kSlotsV]), end / kSlotsV & 1u, abort_flag)) {
           for (uint32_t c = 0; c < kChunks; ++c)
             for (uint32_t at = left * 128u + lane * 16u; at < kChunk; at += 512u)
               asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(last_at + c * kChunk + at), "r"(0u) : "memory");
@@ -238,55 +288,39 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
         }
         if (*abort_flag) {   // the copies in flight land before shared memory is given up
           mbar_wait_quiet(smem_u32(&q_full), 0);
-          for (uint32_t s = 0; s < kStages; ++s)
-            if (armed & (1u << s)) mbar_wait_quiet(smem_u32(&full_bar[s]), (parity >> s) & 1u);
+          for (uint32_t j = copied_k > kSlotsK ? copied_k - kSlotsK : 0u; j < copied_k; ++j) mbar_wait_quiet(smem_u32(&k_full[j % kSlotsK]), j / kSlotsK & 1u);
+          for (uint32_t j = copied_v > kSlotsV ? copied_v - kSlotsV : 0u; j < copied_v; ++j) mbar_wait_quiet(smem_u32(&v_full[j % kSlotsV]), j / kSlotsV & 1u);
         }
       }
-    } else if (warp == 8) {
+    } else if (warp == 0) {
       // ------------------------------ products ------------------------------
       if (steps > 0) {
         constexpr uint32_t kS = idesc_of(kTile, 0), kY = idesc_of(kD, 1);
-        uint32_t stage = 0, phase = 0;
-        bool ok = wait_all(smem_u32(&q_full), 0, abort_flag) && wait_all(smem_u32(&full_bar[0]), 0, abort_flag);
-        if (ok) {
-#pragma unroll
-          for (uint32_t x = 0; x < 2; ++x)
-            if (tiles[x] > 0) {
-              product_nt<kD>(tmem + x * kTile, smem + x * kBytes, ring, kS);
-              mma_commit(smem_u32(&s_full[x]));
-            }
-          mma_commit(smem_u32(&empty_bar[0]));
-          stage = 1;
-        }
+        const uint32_t leader = elect_one();
+        const uint32_t s_done = smem_u32(&s_full[0]), p_done = smem_u32(&p_full[0]), made = smem_u32(&y_done[0]);
+        uint32_t k_at = 0, k_phase = 0, v_at = 0, v_phase = 0;
+        auto make_s = [&](uint32_t x) {
+          if (x == 0 && !wait_all(smem_u32(&k_full[0]) + 8 * k_at, k_phase, abort_flag)) return false;
+          product_nt<kD>(tmem + x * kTile, smem + x * kBytes, k_ring + k_at * kBytes, kS, leader);
+          commit(s_done + 8 * x, leader);
+          if (x + 1 == count) {
+            commit(smem_u32(&k_empty[0]) + 8 * k_at, leader);
+            if (++k_at == kSlotsK) k_at = 0, k_phase ^= 1u;
+          }
+          return true;
+        };
+        bool ok = wait_all(smem_u32(&q_full), 0, abort_flag) && make_s(0) && (count == 1u || make_s(1));
         for (uint32_t j = 0; ok && j < steps; ++j) {
-          const uint32_t v_stage = stage, v_phase = phase;
-          if (++stage == kStages) stage = 0, phase ^= 1u;
-          const uint32_t k_stage = stage;
-          if (!wait_all(smem_u32(&full_bar[v_stage]), v_phase, abort_flag)) { ok = false; break; }
-          if (j + 1 == steps && left != 0u && !wait_all(smem_u32(&v_clean), 0, abort_flag)) { ok = false; break; }
-          if (j + 1 < steps && !wait_all(smem_u32(&full_bar[k_stage]), phase, abort_flag)) { ok = false; break; }
-#pragma unroll
-          for (uint32_t x = 0; x < 2; ++x) {
-            if (ok && j < tiles[x]) {
-              if (!wait_all(smem_u32(&p_full[x]), j & 1u, abort_flag)) {
-                ok = false;
-              } else {
-                tc_fence_after();
-                product_pn(tmem + 2 * kTile + x * kD, tmem + x * kTile, ring + v_stage * kBytes, kY, j == 0);
-                mma_commit(smem_u32(&y_done[x]));
-                if (j + 1 < tiles[x]) {
-                  product_nt<kD>(tmem + x * kTile, smem + x * kBytes, ring + k_stage * kBytes, kS);
-                  mma_commit(smem_u32(&s_full[x]));
-                }
-              }
-            }
+          ok = wait_all(smem_u32(&v_full[0]) + 8 * v_at, v_phase, abort_flag) && (j + 1 < steps || left == 0u || wait_all(smem_u32(&v_clean), 0, abort_flag));
+          for (uint32_t x = 0; ok && x < count; ++x) {
+            if (!wait_all(p_done + 8 * x, j & 1u, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            product_pn(tmem + 2 * kTile + x * kD, tmem + x * kTile, v_ring + v_at * kBytes, kY, j == 0, leader);
+            commit(made + 8 * x, leader);
+            if (j + 1 < steps) ok = make_s(x);
           }
-          if (!ok) break;
-          mma_commit(smem_u32(&empty_bar[v_stage]));
-          if (j + 1 < steps) {
-            mma_commit(smem_u32(&empty_bar[k_stage]));
-            if (++stage == kStages) stage = 0, phase ^= 1u;
-          }
+          commit(smem_u32(&v_empty[0]) + 8 * v_at, leader);
+          if (++v_at == kSlotsV) v_at = 0, v_phase ^= 1u;
         }
         if (*abort_flag) {   // retire whatever was issued before tensor memory is freed
           __syncwarp();
@@ -294,12 +328,12 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
           mbar_wait_quiet(smem_u32(&drain_bar), 0);
         }
       }
-    } else if (warp < 8) {
+    } else if (warp >= 4) {
       // ------------------------------ softmax ------------------------------
       asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-      const uint32_t x = warp >> 2, quarter = warp & 3u;
+      const uint32_t x = (warp >> 2) - 1u, quarter = warp & 3u;
       const uint32_t lanes = (quarter * 32u) << 16, s_tmem = tmem + lanes + x * kTile, y_tmem = tmem + lanes + 2 * kTile + x * kD;
-      const uint32_t tok = (x ? tok0[1] : tok0[0]) + quarter * 32u + lane, n = x ? tiles[1] : tiles[0];
+      const uint32_t tok = tok_of(x) + quarter * 32u + lane, n = x < count ? steps : 0u;
       // keys that this row sees
       long long sees = q.lk;
       if (a.causal) sees = min(sees, max(0ll, static_cast<long long>(tok) + 1 + shift));
@@ -326,10 +360,10 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[c][i]));
-        const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        // (a row that has seen nothing has m = -inf: its sum and y are zeros, whatever they are multiplied with)
-        const bool move = now > m && (now - m) * to2 > 8.f;
+          for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+        const float now = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+        // (a row that has seen nothing has m = -inf, and zeros for its sum and y; a NaN moves, and stays in both)
+        const bool move = now != m && !((now - m) * to2 <= 8.f);
         if (j == 0) {
           m = now;
         } else if (__any_sync(0xffffffffu, move)) {
@@ -357,8 +391,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
           for (int i = 0; i < 32; ++i) {
             const int c = h * 2 + i / 16, e = (i % 16) * 2;
             float u, w;
-            unpair(fma2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), to22, base2), u, w);
-            u = attn_exp2(u), w = attn_exp2(w);
+            exp2_pair(i, fma2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), to22, base2), u, w);
             sum[i & 1] = add2(sum[i & 1], pair_of(u, w));
             out[i] = halves_of(u, w);
           }
@@ -374,10 +407,10 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
       }
       if (ok && n > 0) ok = wait_all(smem_u32(&y_done[x]), (n - 1) & 1u, abort_flag);
       tc_fence_after();
-      if (ok && (x ? has[1] : has[0])) {
+      if (ok && x < count) {
         const bool some = m != -INFINITY, mine = tok < q.lq;
         const float inv = some ? 1.f / l : 0.f;
-        const uint32_t head = head0 + (p.two_heads ? x : 0u);
+        const uint32_t head = head_of(x);
         __half *out = static_cast<__half *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(head) * a.head;
 #pragma unroll
         for (int c = 0; c < kD / 32; ++c) {
@@ -405,7 +438,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && s_abort) report_status(p.status, B200_ERR_KERNEL_TIMEOUT);
-  if (warp == 8) {
+  if (warp == 0) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
@@ -418,12 +451,15 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
 // through a ring:
 //   keys at rest     X1 = k, X2 = v, Y1 = q, Y2 = gy:   s' = k q^T, dp' = v gy^T,  gv += p' gy,  gk += ds' q
 //   queries at rest  X1 = q, X2 = gy, Y1 = k, Y2 = v:   s = q k^T,  dp = gy v^T,   gq += ds k
-// Transposed where the keys rest, so that p and ds are always the left operand, from tensor memory, where they take the place of s
-// and dp, and a tile in shared memory serves both as the right operand of the first products and of the second.  Eight
-// warps share a tile: a thread has 64 of a row's 128 columns.
-//   order of the products, keys at rest:     gv(i) s(i+1) gk(i) dp(i+1): p(i+1) is made beside the last two, ds(i+1) beside the first two
-//   queries at rest:                         s(i+1) gq(i) dp(i+1), with two buffers for s
-// Bound by the tensor core: 2048 + 1536 clocks per 128 x 128 pairs, against 1024 of the special function units in each.
+// Transposed where the keys rest, so that p and ds are always the left operand, from tensor memory, and a tile in shared memory
+// serves both as the right operand of the first products and of the second.  Eight warps share a tile: a thread has 64 of a
+// row's 128 columns.
+//   keys at rest: the sums take half of tensor memory, so s and dp have one place between them: s(i) is in registers when dp(i) is
+//     issued, and dp(i) is when s(i+1) is.  Order of the products: dp(i) s(i+1) gv(i), dp(i+1) gk(i) ...
+//     (With places of their own, p written over s and ds over dp, s(i+1) waited for gv(i) and that for p(i): 3250 clocks a step.)
+//   queries at rest: s(i+1) dp(i+1) gq(i), ds over dp, which has two buffers
+// Bound by the tensor core, 2048 + 1536 clocks per 128 x 128 pairs, and as much by what shared memory has to read for it; the
+// exponentials are 1024 of the special function units in each, of which exp2_pair takes a part over.
 //
 // p and ds are halves.  p is stored as 2^13 p; ds after a scale by a power of two from the largest |ds| that the norms of gy and v
 // allow, over all that the block sees (keys at rest) or per query: without it the ds of long rows lie below the smallest half.
@@ -436,9 +472,23 @@ struct alignas(64) BwParams {
 };
 
 constexpr uint32_t kBwThreads = 384;
-template <int kD> constexpr uint32_t kBwStages = kD == 128 ? 2u : 4u;
-template <int kD> constexpr uint32_t kBwSmem = (2 + 2 * kBwStages<kD>) * kTile * kD * 2 + 1024;
 constexpr float kPBits = 13.f;
+// Slots of the rings.  Y1 is needed first and given back last, by the product that ends a step: with two slots its copy started a step
+// late, and a step of the gq kernel took 3500 clocks instead of 1900.
+template <int kD> constexpr uint32_t kY1 = kD == 128 ? 3u : 4u;
+template <int kD> constexpr uint32_t kY2 = kD == 128 ? 2u : 3u;
+constexpr uint32_t kStats = 2;
+constexpr uint32_t kBwHead = 3072;   // bytes in front of the tiles; with 7 tiles of 32 KB that is all there is
+template <int kD> constexpr uint32_t kBwSmem = kBwHead + (2 + kY1<kD> + kY2<kD>) * kTile * kD * 2;
+
+struct BwShared {
+  float stat[kStats][2][kTile];      // keys at rest: 13 - lse log2(e), and -delta scaled, of the queries that pass by
+  uint64_t x_full, full1[4], ready1[4], empty1[4], full2[4], ready2[4], empty2[4], s_full, s_read, dp_full[2], dp_read, p_full, ds_full[2], acc_done, drain;
+  float top[3][kBwThreads / 32];
+  uint32_t tmem, at[2];
+  int abort;
+};
+static_assert(sizeof(BwShared) <= kBwHead, "no room");
 
 // The power of two that takes the largest |ds| possible to at most 2^14.  |dp - delta| <= |gy| |v| + |delta|.
 __device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) {
@@ -447,35 +497,44 @@ __device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) 
   return exp2f(fminf(fmaxf(13.f - ceilf(log2f(bound)), -100.f), 100.f));
 }
 
+// A position in a ring.
+template <uint32_t kSlots>
+struct Slot {
+  uint32_t at = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == kSlots) at = 0, phase ^= 1u;
+  }
+};
+
+// Four floats of shared memory as two pairs.
+__device__ __forceinline__ void stat4(const float *p, f32x2 &a, f32x2 &b) {
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(p);
+  a = v.x, b = v.y;
+}
+
 template <int kD, bool kKeys>
 __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __grid_constant__ BwParams p) {
-  constexpr uint32_t kBytes = kTile * kD * 2, kStages = kBwStages<kD>, kChunks = kD / 64;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t x_full, full_bar[kStages], ready_bar[kStages], empty_bar[kStages], s_full[2], dp_full, p_full, ds_full, acc_done, drain_bar;
-  __shared__ __align__(16) float s_stat[kKeys ? kStages : 1][2][kTile];   // -lse log2(e) + 13, and -delta, scaled
-  __shared__ float s_max[3][kBwThreads / 32];
-  __shared__ uint32_t tmem_slot, s_at[2];
-  __shared__ int s_abort;
+  constexpr uint32_t kBytes = kTile * kD * 2, kChunks = kD / 64, kSlots1 = kY1<kD>, kSlots2 = kY2<kD>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   pdl_release_next();
+  BwShared &sh = *reinterpret_cast<BwShared *>(smem_raw);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem + 2 * kBytes;
-  volatile int *abort_flag = &s_abort;
+  const uint32_t smem = smem_u32(smem_raw) + kBwHead, ring1 = smem + 2 * kBytes, ring2 = ring1 + kSlots1 * kBytes;
+  volatile int *abort_flag = &sh.abort;
   const AttnArgs &a = p.a;
-  if (threadIdx.x == 9u * 32u) {
+  if (threadIdx.x == 32u) {
     for (const CUtensorMap *m : {&p.x1, &p.x2, &p.y1, &p.y2}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(m)) : "memory");
   }
   if (threadIdx.x == 0) {
-    s_abort = 0;
-    mbar_init(smem_u32(&x_full), 1);
-    for (uint32_t i = 0; i < kStages; ++i)
-      mbar_init(smem_u32(&full_bar[i]), 1), mbar_init(smem_u32(&ready_bar[i]), 1), mbar_init(smem_u32(&empty_bar[i]), 1);
-    mbar_init(smem_u32(&s_full[0]), 1), mbar_init(smem_u32(&s_full[1]), 1), mbar_init(smem_u32(&dp_full), 1);
-    mbar_init(smem_u32(&p_full), 8), mbar_init(smem_u32(&ds_full), 8);
-    mbar_init(smem_u32(&acc_done), 1), mbar_init(smem_u32(&drain_bar), 1);
+    sh.abort = 0;
+    for (uint64_t *one : {&sh.x_full, &sh.s_full, &sh.dp_full[0], &sh.dp_full[1], &sh.acc_done, &sh.drain}) mbar_init(smem_u32(one), 1);
+    for (uint32_t i = 0; i < 4; ++i)
+      for (uint64_t *one : {&sh.full1[i], &sh.ready1[i], &sh.empty1[i], &sh.full2[i], &sh.ready2[i], &sh.empty2[i]}) mbar_init(smem_u32(one), 1);
+    for (uint64_t *warps : {&sh.s_read, &sh.dp_read, &sh.p_full, &sh.ds_full[0], &sh.ds_full[1]}) mbar_init(smem_u32(warps), 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait_previous();
@@ -483,11 +542,11 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
   // heaviest first: the first keys of a causal sequence are seen by the most queries, its last queries see the most keys
   const uint32_t column = blockIdx.x % p.columns, nth = blockIdx.x / p.columns;
   uint32_t seq, tile;
-  const bool any = attn_find_tile<kKeys>(a, kKeys ? nth : p.tiles - 1u - nth, 1, kTile, s_at, seq, tile);
+  const bool any = attn_find_tile<kKeys>(a, kKeys ? nth : p.tiles - 1u - nth, 1, kTile, sh.at, seq, tile);
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  constexpr uint32_t kDp = kKeys ? kTile : 2 * kTile;                          // columns of dp
-  constexpr uint32_t kAcc1 = 2 * kTile, kAcc2 = kKeys ? 2 * kTile + kD : 3 * kTile;   // gv; gk or gq
+  const uint32_t tmem = sh.tmem;
+  // columns of tensor memory.  Keys at rest: s and then dp, p, ds, two sums; queries at rest: s, two of dp and ds, the sum
+  constexpr uint32_t kP = kTile, kDs = kTile + 64u, kDp = kTile, kAcc1 = 2 * kTile, kAcc2 = kKeys ? 2 * kTile + kD : 3 * kTile;
 
   if (any) {
     const AttnSeq q = attn_seq(a, seq);
@@ -531,130 +590,163 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
         dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, o));
         vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
       }
-      if (lane == 0) s_max[0][warp] = gm, s_max[1][warp] = dm, s_max[2][warp] = vm;
+      if (lane == 0) sh.top[0][warp] = gm, sh.top[1][warp] = dm, sh.top[2][warp] = vm;
       __syncthreads();
 #pragma unroll
-      for (uint32_t w = 0; w < kBwThreads / 32; ++w) gm = fmaxf(gm, s_max[0][w]), dm = fmaxf(dm, s_max[1][w]), vm = fmaxf(vm, s_max[2][w]);
+      for (uint32_t w = 0; w < kBwThreads / 32; ++w) gm = fmaxf(gm, sh.top[0][w]), dm = fmaxf(dm, sh.top[1][w]), vm = fmaxf(vm, sh.top[2][w]);
       ds_scale = scale_of(gm, vm, dm);
     }
 
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 9) {
+    // 168 registers a thread at launch: 56 + 2 * 224 = 3 * 168
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 1) {
       // ------------------------------ copies ------------------------------
       if (steps > 0) {
-        uint32_t stage = 0, phase = 0, armed = 0, parity = 0;
+        const int x_row = (kKeys ? q.k0 : q.q0) + row0, x_head = kKeys ? kv_head : q_head;
         if (lane == 0) {
-          mbar_arrive_expect_tx(smem_u32(&x_full), 2 * kBytes);
+          mbar_arrive_expect_tx(smem_u32(&sh.x_full), 2 * kBytes);
           for (uint32_t c = 0; c < kChunks; ++c) {
-            const int head = kKeys ? kv_head : q_head, row = (kKeys ? q.k0 : q.q0) + row0;
-            tma_load_3d(smem + c * kChunk, &p.x1, smem_u32(&x_full), c * 64, head, row);
-            tma_load_3d(smem + kBytes + c * kChunk, &p.x2, smem_u32(&x_full), c * 64, head, row);
+            tma_load_3d(smem + c * kChunk, &p.x1, smem_u32(&sh.x_full), c * 64, x_head, x_row);
+            tma_load_3d(smem + kBytes + c * kChunk, &p.x2, smem_u32(&sh.x_full), c * 64, x_head, x_row);
           }
         }
         __syncwarp();
-        uint32_t g = 0, t = 0;
-        for (uint32_t i = 0; i < steps; ++i) {
-          if (!wait_all(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) break;
-          const uint32_t bar = smem_u32(&full_bar[stage]), dst = ring + stage * 2 * kBytes;
+        Slot<kSlots1> s1;
+        Slot<kSlots2> s2;
+        uint32_t g = 0, t = 0, armed1 = 0, armed2 = 0, parity1 = 0, parity2 = 0;
+        auto copy = [&](const CUtensorMap *map, uint32_t bar, uint32_t dst) {
           if (lane == 0) {
-            mbar_arrive_expect_tx(bar, 2 * kBytes);
             const int head = kKeys ? q_head + g : kv_head, row = (kKeys ? q.q0 : q.k0) + from + t * kTile;
-            for (uint32_t c = 0; c < kChunks; ++c) {
-              tma_load_3d(dst + c * kChunk, &p.y1, bar, c * 64, head, row);
-              tma_load_3d(dst + kBytes + c * kChunk, &p.y2, bar, c * 64, head, row);
-            }
+            mbar_arrive_expect_tx(bar, kBytes);
+            for (uint32_t c = 0; c < kChunks; ++c) tma_load_3d(dst + c * kChunk, map, bar, c * 64, head, row);
           }
           __syncwarp();
-          armed |= 1u << stage;
-          parity = (parity & ~(1u << stage)) | (phase << stage);
+        };
+        for (uint32_t i = 0; i < steps; ++i) {
+          if (!wait_all(smem_u32(&sh.empty1[s1.at]), s1.phase ^ 1u, abort_flag)) break;
+          copy(&p.y1, smem_u32(&sh.full1[s1.at]), ring1 + s1.at * kBytes);
+          armed1 |= 1u << s1.at, parity1 = (parity1 & ~(1u << s1.at)) | (s1.phase << s1.at);
+          if (!wait_all(smem_u32(&sh.empty2[s2.at]), s2.phase ^ 1u, abort_flag)) break;
+          copy(&p.y2, smem_u32(&sh.full2[s2.at]), ring2 + s2.at * kBytes);
+          armed2 |= 1u << s2.at, parity2 = (parity2 & ~(1u << s2.at)) | (s2.phase << s2.at);
           if (++t == per) t = 0, ++g;
-          if (++stage == kStages) stage = 0, phase ^= 1u;
+          s1.next(), s2.next();
         }
-        if (*abort_flag) {
-          mbar_wait_quiet(smem_u32(&x_full), 0);
-          for (uint32_t s = 0; s < kStages; ++s)
-            if (armed & (1u << s)) mbar_wait_quiet(smem_u32(&full_bar[s]), (parity >> s) & 1u);
-        }
-      }
-    } else if (warp == 10) {
-      // ------------------------------ what a tile needs before use: its rows' numbers, zeros behind its last row ------------------------------
-      uint32_t stage = 0, phase = 0, g = 0, t = 0;
-      for (uint32_t i = 0; i < steps; ++i) {
-        if (!wait_all(smem_u32(&full_bar[stage]), phase, abort_flag)) break;
-        if constexpr (kKeys) {
-          const float f = ds_scale * exp2f(-kPBits);
-#pragma unroll
-          for (uint32_t c = lane; c < kTile; c += 32u) {
-            const uint32_t tok = from + t * kTile + c;
-            const unsigned long long at = stat + static_cast<unsigned long long>(g) * a.rows_q + tok;
-            const float lse = tok < q.lq ? a.lse[at] : -INFINITY;
-            s_stat[stage][0][c] = lse == -INFINITY ? lse : kPBits - lse * kLog2e;
-            s_stat[stage][1][c] = tok < q.lq ? -a.delta[at] * f : 0.f;
+        if (*abort_flag) {   // the copies in flight land before shared memory is given up
+          mbar_wait_quiet(smem_u32(&sh.x_full), 0);
+          for (uint32_t s = 0; s < 4; ++s) {
+            if (armed1 & (1u << s)) mbar_wait_quiet(smem_u32(&sh.full1[s]), (parity1 >> s) & 1u);
+            if (armed2 & (1u << s)) mbar_wait_quiet(smem_u32(&sh.full2[s]), (parity2 >> s) & 1u);
           }
         }
-        if (t + 1 == per && left != 0u) {
-          const uint32_t base = ring + stage * 2 * kBytes;
-          for (uint32_t c = 0; c < 2 * kChunks; ++c)
-            for (uint32_t at = left * 128u + lane * 16u; at < kChunk; at += 512u)
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + c * kChunk + at), "r"(0u) : "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ready_bar[stage]));
-        if (++t == per) t = 0, ++g;
-        if (++stage == kStages) stage = 0, phase ^= 1u;
       }
-    } else if (warp == 8) {
+    } else if (warp == 2) {
+      // -------------------- what a tile needs before use: its rows' numbers, zeros behind its last row --------------------
+      Slot<kSlots1> s1;
+      Slot<kSlots2> s2;
+      uint32_t g = 0, t = 0;
+      auto clean = [&](uint32_t base) {   // p and ds are zero there, but zero times an infinity is not
+        for (uint32_t c = 0; c < kChunks; ++c)
+          for (uint32_t at = left * 128u + lane * 16u; at < kChunk; at += 512u)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + c * kChunk + at), "r"(0u) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      };
+      const float f = ds_scale * exp2f(-kPBits);
+      for (uint32_t i = 0; i < steps; ++i) {
+        if constexpr (kKeys) {
+          float lse[4], delta[4];
+#pragma unroll
+          for (uint32_t c = 0; c < 4; ++c) {
+            const uint32_t tok = from + t * kTile + c * 32u + lane;
+            const unsigned long long at = stat + static_cast<unsigned long long>(g) * a.rows_q + tok;
+            lse[c] = tok < q.lq ? a.lse[at] : -INFINITY;
+            delta[c] = tok < q.lq ? a.delta[at] : 0.f;
+          }
+          // the numbers of two steps ago are done with when that step's ds is
+          if (i >= kStats && !wait_all(smem_u32(&sh.ds_full[i & 1u]), ((i - kStats) >> 1) & 1u, abort_flag)) break;
+#pragma unroll
+          for (uint32_t c = 0; c < 4; ++c) {
+            sh.stat[i % kStats][0][c * 32u + lane] = lse[c] == -INFINITY ? lse[c] : kPBits - lse[c] * kLog2e;
+            sh.stat[i % kStats][1][c * 32u + lane] = -delta[c] * f;
+          }
+        }
+        const bool cut = t + 1 == per && left != 0u;
+        if (!wait_all(smem_u32(&sh.full1[s1.at]), s1.phase, abort_flag)) break;
+        if (cut) clean(ring1 + s1.at * kBytes);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.ready1[s1.at]));
+        if (!wait_all(smem_u32(&sh.full2[s2.at]), s2.phase, abort_flag)) break;
+        if (cut) clean(ring2 + s2.at * kBytes);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.ready2[s2.at]));
+        if (++t == per) t = 0, ++g;
+        s1.next(), s2.next();
+      }
+    } else if (warp == 0) {
       // ------------------------------ products ------------------------------
       if (steps > 0) {
         constexpr uint32_t kS = idesc_of(kTile, 0), kG = idesc_of(kD, 1);
-        uint32_t stage = 0, phase = 0;
+        const uint32_t leader = elect_one();
+        Slot<kSlots1> s1;   // of the next step
+        Slot<kSlots2> s2;
         // (`ready` follows `full`, which is what orders the copies before the products)
-        auto tile_ready = [&](uint32_t s, uint32_t ph) { return wait_all(smem_u32(&ready_bar[s]), ph, abort_flag) && wait_all(smem_u32(&full_bar[s]), ph, abort_flag); };
-        bool ok = wait_all(smem_u32(&x_full), 0, abort_flag) && tile_ready(0, 0);
-        if (ok) {
-          product_nt<kD>(tmem, smem, ring, kS);
-          mma_commit(smem_u32(&s_full[0]));
-          product_nt<kD>(tmem + kDp, smem + kBytes, ring + kBytes, kS);
-          mma_commit(smem_u32(&dp_full));
-        }
-        for (uint32_t i = 0; ok && i < steps; ++i) {
-          const uint32_t y1 = ring + stage * 2 * kBytes, y2 = y1 + kBytes, this_stage = stage;
-          if (++stage == kStages) stage = 0, phase ^= 1u;
-          const uint32_t next = ring + stage * 2 * kBytes;
-          const bool more = i + 1 < steps;
-          if constexpr (kKeys) {
-            if (!wait_all(smem_u32(&p_full), i & 1u, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            product_pn2(tmem + kAcc1, tmem, y2, kG, i == 0);
-          }
-          if (more) {
-            if (!tile_ready(stage, phase)) { ok = false; break; }
-            const uint32_t b = kKeys ? 0u : (i + 1) & 1u;
-            product_nt<kD>(tmem + b * kTile, smem, next, kS);
-            mma_commit(smem_u32(&s_full[b]));
-          }
-          if (!wait_all(smem_u32(&ds_full), i & 1u, abort_flag)) { ok = false; break; }
+        auto make_s = [&]() {
+          if (!wait_all(smem_u32(&sh.ready1[s1.at]), s1.phase, abort_flag) || !wait_all(smem_u32(&sh.full1[s1.at]), s1.phase, abort_flag)) return false;
+          product_nt<kD>(tmem, smem, ring1 + s1.at * kBytes, kS, leader);
+          commit(smem_u32(&sh.s_full), leader);
+          return true;
+        };
+        auto make_dp = [&](uint32_t d, uint32_t b) {
+          if (!wait_all(smem_u32(&sh.ready2[s2.at]), s2.phase, abort_flag) || !wait_all(smem_u32(&sh.full2[s2.at]), s2.phase, abort_flag)) return false;
+          product_nt<kD>(tmem + d, smem + kBytes, ring2 + s2.at * kBytes, kS, leader);
+          commit(smem_u32(&sh.dp_full[b]), leader);
+          if (!kKeys) commit(smem_u32(&sh.empty2[s2.at]), leader);
+          return true;
+        };
+        auto heard = [&](uint64_t *bar, uint32_t parity) {
+          if (!wait_all(smem_u32(bar), parity, abort_flag)) return false;
           tc_fence_after();
-          product_pn2(tmem + kAcc2, tmem + kDp, y1, kG, i == 0);
-          mma_commit(smem_u32(&empty_bar[this_stage]));
-          if (more) {
-            product_nt<kD>(tmem + kDp, smem + kBytes, next + kBytes, kS);
-            mma_commit(smem_u32(&dp_full));
+          return true;
+        };
+        bool ok = wait_all(smem_u32(&sh.x_full), 0, abort_flag) && make_s();
+        if constexpr (kKeys) {
+          ok = ok && heard(&sh.s_read, 0) && make_dp(0, 0);
+          for (uint32_t i = 0; ok && i < steps; ++i) {
+            const uint32_t at1 = s1.at, at2 = s2.at;
+            const bool more = i + 1 < steps;
+            s1.next(), s2.next();
+            if (more) ok = heard(&sh.dp_read, i & 1u) && make_s();
+            if (!ok || !heard(&sh.p_full, i & 1u)) { ok = false; break; }
+            product_pn(tmem + kAcc1, tmem + kP, ring2 + at2 * kBytes, kG, i == 0, leader);
+            commit(smem_u32(&sh.empty2[at2]), leader);
+            if (more) ok = heard(&sh.s_read, (i + 1) & 1u) && make_dp(0, 0);
+            if (!ok || !heard(&sh.ds_full[i & 1u], (i >> 1) & 1u)) { ok = false; break; }
+            product_pn(tmem + kAcc2, tmem + kDs, ring1 + at1 * kBytes, kG, i == 0, leader);
+            commit(smem_u32(&sh.empty1[at1]), leader);
+          }
+        } else {
+          ok = ok && make_dp(kDp, 0);
+          for (uint32_t i = 0; ok && i < steps; ++i) {
+            const uint32_t at1 = s1.at, b = i & 1u;
+            s1.next(), s2.next();
+            if (i + 1 < steps) ok = heard(&sh.s_read, b) && make_s() && make_dp(kDp + (b ^ 1u) * kTile, b ^ 1u);
+            if (!ok || !heard(&sh.ds_full[b], (i >> 1) & 1u)) { ok = false; break; }
+            product_pn<true>(tmem + kAcc2, tmem + kDp + b * kTile, ring1 + at1 * kBytes, kG, i == 0, leader);
+            commit(smem_u32(&sh.empty1[at1]), leader);
           }
         }
-        if (ok) mma_commit(smem_u32(&acc_done));
-        if (*abort_flag) {
+        if (ok) commit(smem_u32(&sh.acc_done), leader);
+        if (*abort_flag) {   // retire whatever was issued before tensor memory is freed
           __syncwarp();
-          mma_commit(smem_u32(&drain_bar));
-          mbar_wait_quiet(smem_u32(&drain_bar), 0);
+          mma_commit(smem_u32(&sh.drain));
+          mbar_wait_quiet(smem_u32(&sh.drain), 0);
         }
       }
-    } else if (warp < 8) {
+    } else if (warp >= 4) {
       // ------------------------------ p and ds ------------------------------
       asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-      const uint32_t half = warp >> 2, quarter = warp & 3u, col0 = half * 64u;
-      const uint32_t lanes = (quarter * 32u) << 16;
+      const uint32_t half = (warp >> 2) - 1u, quarter = warp & 3u, col0 = half * 64u;
+      const uint32_t lanes = (quarter * 32u) << 16, s_tmem = tmem + lanes + col0;
       const uint32_t row = row0 + quarter * 32u + lane;
       const float to2 = a.scale * kLog2e;
       float base = 0.f, minus_delta = 0.f;
@@ -670,19 +762,24 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
         if (a.causal) sees = min(sees, max(0ll, static_cast<long long>(row) + 1 + shift));
       }
       const float f = kKeys ? ds_scale * exp2f(-kPBits) : ds_scale;
-      const f32x2 to22 = pair_of(to2, to2), f2 = pair_of(f, f);
-      uint32_t stage = 0, phase = 0, t = 0;
+      const f32x2 to22 = pair_of(to2, to2), f2 = pair_of(f, f), base2 = pair_of(base, base), minus_delta2 = pair_of(minus_delta, minus_delta);
+      Slot<kSlots1> s1;
+      uint32_t t = 0;
       bool ok = true;
       for (uint32_t i = 0; i < steps; ++i) {
-        const uint32_t b = kKeys ? 0u : i & 1u, s_tmem = tmem + lanes + b * kTile + col0, dp_tmem = tmem + lanes + kDp + col0;
-        if (kKeys && !wait_all(smem_u32(&ready_bar[stage]), phase, abort_flag)) { ok = false; break; }
-        if (!wait_all(smem_u32(&s_full[b]), (kKeys ? i : i >> 1) & 1u, abort_flag)) { ok = false; break; }
+        const uint32_t b = i & 1u, dp_tmem = tmem + lanes + (kKeys ? 0u : kDp + b * kTile) + col0;
+        const float *stat0 = sh.stat[i % kStats][0] + col0, *stat1 = sh.stat[i % kStats][1] + col0;
+        if (kKeys && !wait_all(smem_u32(&sh.ready1[s1.at]), s1.phase, abort_flag)) { ok = false; break; }
+        if (!wait_all(smem_u32(&sh.s_full), i & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
         uint32_t s[2][32];
         tmem_ld32_issue(s_tmem, s[0]);
         tmem_ld32_issue(s_tmem + 32, s[1]);
         tmem_ld_wait(s[0]);
         tmem_ld_wait(s[1]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.s_read));
         // columns of this thread that its row has no part in: [0, skip) where queries pass by, [skip, 64) where keys do
         int skip;
         if constexpr (kKeys) {
@@ -698,53 +795,68 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
             for (int e = 0; e < 32; ++e)
               if (kKeys ? c * 32 + e < skip : c * 32 + e >= skip) s[c][e] = 0xff800000u;
         }
-        uint32_t out[32];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            f32x2 add = pair_of(base, base);
-            if constexpr (kKeys) add = *reinterpret_cast<const f32x2 *>(&s_stat[stage][0][col0 + c * 32 + e]);
-            float u, w;
-            unpair(fma2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), to22, add), u, w);
-            u = attn_exp2(u), w = attn_exp2(w);
-            s[c][e] = __float_as_uint(u), s[c][e + 1] = __float_as_uint(w);
-            if constexpr (kKeys) out[c * 16 + e / 2] = halves_of(u, w);
+          for (int e = 0; e < 32; e += 4) {
+            f32x2 add[2] = {base2, base2};
+            if constexpr (kKeys) stat4(stat0 + c * 32 + e, add[0], add[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int at = e + 2 * k;
+              float u, w;
+              exp2_pair(at / 2, fma2(pair_of(__uint_as_float(s[c][at]), __uint_as_float(s[c][at + 1])), to22, add[k]), u, w);
+              s[c][at] = __float_as_uint(u), s[c][at + 1] = __float_as_uint(w);
+            }
           }
-        if constexpr (kKeys) {
-          tmem_st32(s_tmem, out);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&p_full));
-        }
-        if (!wait_all(smem_u32(&dp_full), i & 1u, abort_flag)) { ok = false; break; }
+        if (!wait_all(smem_u32(&sh.dp_full[kKeys ? 0u : b]), (kKeys ? i : i >> 1) & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        uint32_t d[2][32];
+        uint32_t d[2][32], out[32];
         tmem_ld32_issue(dp_tmem, d[0]);
         tmem_ld32_issue(dp_tmem + 32, d[1]);
         tmem_ld_wait(d[0]);
         tmem_ld_wait(d[1]);
+        if constexpr (kKeys) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.dp_read));
+          // (dp(i) is issued behind gv(i - 1), so p(i - 1) is read)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) out[e] = halves_of(__uint_as_float(s[e >> 4][(e & 15) * 2]), __uint_as_float(s[e >> 4][(e & 15) * 2 + 1]));
+          tmem_st32(tmem + lanes + kP + half * 32u, out);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            f32x2 add = pair_of(minus_delta, minus_delta);
-            if constexpr (kKeys) add = *reinterpret_cast<const f32x2 *>(&s_stat[stage][1][col0 + c * 32 + e]);
-            float u, w;
-            unpair(mul2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])),
-                        fma2(pair_of(__uint_as_float(d[c][e]), __uint_as_float(d[c][e + 1])), f2, add)), u, w);
-            out[c * 16 + e / 2] = halves_of(u, w);
+          for (int e = 0; e < 32; e += 4) {
+            f32x2 add[2] = {minus_delta2, minus_delta2};
+            if constexpr (kKeys) stat4(stat1 + c * 32 + e, add[0], add[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int at = e + 2 * k;
+              float u, w;
+              unpair(mul2(pair_of(__uint_as_float(s[c][at]), __uint_as_float(s[c][at + 1])),
+                          fma2(pair_of(__uint_as_float(d[c][at]), __uint_as_float(d[c][at + 1])), f2, add[k])), u, w);
+              out[c * 16 + at / 2] = halves_of(u, w);
+            }
           }
-        tmem_st32(dp_tmem, out);
+        if constexpr (kKeys) {   // gk(i - 1) has read its ds
+          if (i > 0 && !wait_all(smem_u32(&sh.empty1[(i - 1) % kSlots1]), ((i - 1) / kSlots1) & 1u, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+        }
+        tmem_st32(kKeys ? tmem + lanes + kDs + half * 32u : dp_tmem, out);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ds_full));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.ds_full[b]));
         if (++t == per) t = 0;
-        if (++stage == kStages) stage = 0, phase ^= 1u;
+        s1.next();
       }
-      if (ok && steps > 0) ok = wait_all(smem_u32(&acc_done), 0, abort_flag);
+      if (ok && steps > 0) ok = wait_all(smem_u32(&sh.acc_done), 0, abort_flag);
       tc_fence_after();
       if (ok) {
         // keys at rest: gv by the first four warps, gk by the others; queries at rest: half of gq's columns each
@@ -788,8 +900,8 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0 && s_abort) report_status(p.status, B200_ERR_KERNEL_TIMEOUT);
-  if (warp == 8) {
+  if (threadIdx.x == 0 && sh.abort) report_status(p.status, B200_ERR_KERNEL_TIMEOUT);
+  if (warp == 0) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }

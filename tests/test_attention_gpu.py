@@ -427,3 +427,27 @@ def test_refusals(ctx):
     # no keys at all: rows of zeros
     ctx.attention_fw(2, p.plan(rows_k=0, k_starts=None, k_lens=None), a[0], None, None, a[3], a[4])
     assert (p.y == 0.0).all() and (p.lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32"])
+@pytest.mark.parametrize("rows", [200, 1])
+def test_nans_are_not_lost(ctx, mode, rows):
+    """A NaN in a key reaches the queries that see that key, all of them and in y no others; one in a query reaches that query's y alone."""
+    for column in list(range(0, 16)) + [77, 130]:
+        at = packed([200])
+        p = Problem(mode, 64, 2, 1, at if rows > 1 else [(0, 1)], at, True, seed=23)
+        p.k[column, 0, 5] = NAN
+        p.forward(ctx)
+        hit = torch.zeros(rows, dtype=torch.bool, device="cuda")
+        hit[column if rows > 1 else 0:] = True
+        assert torch.equal(p.y[:rows].isnan().all(2).all(1), hit) and torch.equal(p.y[:rows].isnan().any(2).any(1), hit)
+        if rows > 1:
+            p.backward(ctx)
+            assert p.gq[hit].isnan().all() and p.gk[0, 0].isnan().all() and p.gv[0].isnan().all()
+            p = Problem(mode, 64, 2, 1, at, at, True, seed=24)
+            p.q[column, 1, 3] = NAN
+            p.forward(ctx)
+            assert p.y[column, 1].isnan().all() and not p.y[column, 0].isnan().any()
+            assert not p.y[torch.arange(200, device="cuda") != column].isnan().any()
+            p.backward(ctx)
+            assert p.gq[column, 1].isnan().all() and not p.gq[:, 0].isnan().any() and p.gv[:column + 1].isnan().all()
