@@ -1,13 +1,14 @@
 // Attention of a few queries per sequence against many keys: a step of generation, forward only.
 //
 // Bound by the cache, which is read once: 16 rows (queries times the heads of a group) share a key head's keys, and a 16-row
-// mma.sync product costs less than its operands take to arrive.  A sequence's keys are cut over the blocks of a
-// cluster and over the four warps of a block; every warp has a ring of its own, three steps deep, fed by cp.async,
-// so that no warp waits for another while the keys stream.  Each keeps a running softmax; the parts are joined in
-// shared memory and then across the cluster through distributed shared memory, in rank order: one launch, no scratch,
-// the same bits every run.
+// mma.sync product costs less than its operands take to arrive, if little stands beside it.  So copies' addresses are one addition each, the
+// queries stay in registers, masks are looked at in steps that need one, and y is rescaled only when the running maximum moves.
+// (With addresses formed anew 16 keys took 860 instructions.  One bulk copy per row instead: an SM starts one in 30 clocks, which is
+// 8 bytes a clock.)
+// A sequence's keys are cut over the blocks of a cluster and over the four warps of a block; every warp has a ring of its own, so that no
+// warp waits for another while the keys stream.  Each keeps a running softmax; the parts are joined in shared memory and then across
+// the cluster through distributed shared memory, in rank order: one launch, no scratch, the same bits every run.
 #include <algorithm>
-#include <atomic>
 
 #include "attention_mma.cuh"
 #include "tcgen05.cuh"
@@ -15,13 +16,15 @@
 namespace b200 {
 namespace {
 
-constexpr uint32_t kWarps = 4, kThreads = kWarps * 32, kStages = 3;
+constexpr uint32_t kWarps = 4, kThreads = kWarps * 32;
 constexpr uint32_t kMaxSplits = 16;
 template <typename T> constexpr int kStep = sizeof(T) == 2 ? 16 : 8;   // keys per step of a warp
-template <typename T, int kD> constexpr uint32_t kWarpBytes = kStages * 2 * kStep<T> * kPitch<T, kD> * sizeof(T);
+template <typename T, int kD> constexpr uint32_t kRing = sizeof(T) * kD > 512 ? 2 : 3;           // steps in a warp's ring
+template <typename T, int kD> constexpr uint32_t kWarpBytes = kRing<T, kD> * 2 * kStep<T> * kPitch<T, kD> * sizeof(T);
+template <typename T, int kD> constexpr uint32_t kQueryBytes = (sizeof(T) == 2 ? 1 : 2) * 16 * kPitch<T, kD> * sizeof(T);   // fp32: hi and lo
 // the ring, which the parts of the warps take over
 template <typename T, int kD>
-constexpr uint32_t kSmem = std::max<uint32_t>(kWarps * kWarpBytes<T, kD>, kWarps * 16 * kD * 4) + 16 * kPitch<T, kD> * sizeof(T);
+constexpr uint32_t kSmem = std::max<uint32_t>(kWarps * kWarpBytes<T, kD>, kWarps * 16 * kD * 4) + kQueryBytes<T, kD>;
 
 __device__ __forceinline__ float ld_cluster(uint32_t at) {
   float v;
@@ -34,10 +37,85 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
   return v;
 }
 
+// s[16 rows][8 NT] = q k^T.  Halves: q in registers.
+template <int kD, int NT>
+__device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&qf)[kD / 16][4], const __half *k) {
+  constexpr int P = kPitch<__half, kD>;
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint32_t ya = smem_at(k) + (((lane & 7u) + (lane >> 4) * 8u) * P + ((lane >> 3) & 1u) * 8u) * 2u;
+  float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};   // two chains of sums for each tile of eight keys
+  static_assert(NT == 2, "16 keys a step");
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < kD / 16; ++kk) {
+    uint32_t b[4];
+    ldsm4(b, ya + kk * 32);
+    if (kk & 1) {
+      mma_f16(even, qf[kk], b[0], b[1]);
+      mma_f16(odd, qf[kk], b[2], b[3]);
+    } else {
+      mma_f16(s[0], qf[kk], b[0], b[1]);
+      mma_f16(s[1], qf[kk], b[2], b[3]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[0][i] += even[i], s[1][i] += odd[i];
+}
+// fp32: q split beforehand into planes hi and lo.
+template <int kD, int NT, int kPass>
+__device__ __forceinline__ void scores(float (&s)[NT][4], const float *q_hi, const float *q_lo, const float *k) {
+  constexpr int P = kPitch<float, kD>;
+  const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+  const uint32_t *hi = reinterpret_cast<const uint32_t *>(q_hi) + g * P + t, *lo = reinterpret_cast<const uint32_t *>(q_lo) + g * P + t;
+  const float *ka = k + g * P + t;
+  static_assert(NT == 1, "8 keys a step");
+  float c[3][4] = {};   // hi hi, and a chain for either small term
+#pragma unroll 4
+  for (int kk = 0; kk < kD / 8; ++kk) {
+    const uint32_t ah[4] = {hi[kk * 8], hi[8 * P + kk * 8], hi[kk * 8 + 4], hi[8 * P + kk * 8 + 4]};
+    uint32_t bh[2], bl[2];
+    split<kPass>(ka[kk * 8], bh[0], bl[0]);
+    split<kPass>(ka[kk * 8 + 4], bh[1], bl[1]);
+    if constexpr (kPass == 3) {
+      const uint32_t al[4] = {lo[kk * 8], lo[8 * P + kk * 8], lo[kk * 8 + 4], lo[8 * P + kk * 8 + 4]};
+      mma_tf32(c[1], al, bh[0], bh[1]);
+      mma_tf32(c[2], ah, bl[0], bl[1]);
+    }
+    mma_tf32(c[0], ah, bh[0], bh[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[0][i] = c[0][i] + (c[1][i] + c[2][i]);
+}
+
+// y += p v of one step.  Halves: summed by the tensor core (which truncates: 16384 keys lose 3e-5 of a sum, a tenth of its rounding).
+template <int kD, int kPass>
+__device__ __forceinline__ void add_values(float (&acc)[kD / 8][4], const float (&p)[2][4], const __half *v) {
+  constexpr int P = kPitch<__half, kD>;
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint32_t va = smem_at(v) + ((lane & 15u) * P + (lane >> 4) * 8u) * 2u;
+  const uint32_t a[4] = {half2_of(p[0][0], p[0][1]), half2_of(p[0][2], p[0][3]), half2_of(p[1][0], p[1][1]), half2_of(p[1][2], p[1][3])};
+#pragma unroll
+  for (int n = 0; n < kD / 8; n += 2) {
+    uint32_t b[4];
+    ldsm4t(b, va + n * 16);
+    mma_f16(acc[n], a, b[0], b[1]);
+    mma_f16(acc[n + 1], a, b[2], b[3]);
+  }
+}
+template <int kD, int kPass>
+__device__ __forceinline__ void add_values(float (&acc)[kD / 8][4], const float (&p)[1][4], const float *v) {
+  product_py<kD, kD, 1, kPass>(acc, p, v, 0, 1.f, 1.f);
+}
+
 template <typename T, int kD, int kPass>
 __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, uint32_t row_tiles, uint32_t splits, int wide) {
   pdl_enter();
   constexpr int BN = kStep<T>, NT = BN / 8, P = kPitch<T, kD>;
+  constexpr uint32_t kStages = kRing<T, kD>;
+  constexpr bool kHalf = sizeof(T) == 2;
   extern __shared__ __align__(16) unsigned char s_raw[];
   __shared__ float s_m[kWarps][16], s_l[kWarps][16], s_top[16], s_sum[16], s_weight[kMaxSplits][16];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
@@ -46,8 +124,8 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
   const AttnSeq q = attn_seq(a, seq);
   const uint32_t rows = q.lq * a.group, row0 = row_tile * 16u;
   if (row0 >= rows) return;   // the whole cluster
-  T *sq = reinterpret_cast<T *>(s_raw), *ring = sq + 16 * P;
-  T *mine = ring + warp * (kStages * 2 * BN * P);
+  T *sq = reinterpret_cast<T *>(s_raw), *ring_at = reinterpret_cast<T *>(s_raw + kQueryBytes<T, kD>);
+  T *mine = ring_at + warp * (kStages * 2 * BN * P);
   const T *qb = static_cast<const T *>(a.q) + q.q0 * a.q_ld + static_cast<unsigned long long>(hk) * a.group * a.head;
   const T *kb = static_cast<const T *>(a.k) + q.k0 * a.k_ld + static_cast<unsigned long long>(hk) * a.head;
   const T *vb = static_cast<const T *>(a.v) + q.k0 * a.v_ld + static_cast<unsigned long long>(hk) * a.head;
@@ -63,30 +141,75 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
   const uint32_t from = min(rank * per, rounds) * kRound, to = min(keys, min((rank + 1) * per, rounds) * kRound);
   const uint32_t first = from + warp * BN, steps = first < to ? (to - first + kRound - 1) / kRound : 0u;
 
+  // Copies of a step: 32 lanes take whole rows or parts of them, 16 bytes each; a lane keeps its column and adds row strides.
+  constexpr uint32_t kPer = kD * sizeof(T) / 16, kLanes = kPer < 32 ? kPer : 32, kRowsAt = 32 / kLanes, kParts = kPer / kLanes;
+  const bool apart = (wide & (kWideK | kWideV)) != (kWideK | kWideV);
+  const uint32_t lane_row = lane / kLanes, lane_col = lane % kLanes * (16 / sizeof(T));
+  const unsigned long long lane_key = first + lane_row;
+  const T *k_from = kb + lane_key * a.k_ld + lane_col, *v_from = vb + lane_key * a.v_ld + lane_col;
+  const unsigned long long k_rows = kRowsAt * a.k_ld, v_rows = kRowsAt * a.v_ld;
+  const uint32_t lane_to = smem_at(mine + lane_row * P + lane_col);
+  uint32_t load_at = 0;
+  auto copy_rows = [&](uint32_t to_at, const T *from_at, unsigned long long stride, uint32_t have) {
+#pragma unroll
+    for (uint32_t i = 0; i < BN / kRowsAt; ++i) {
+#pragma unroll
+      for (uint32_t part = 0; part < kParts; ++part) {
+        const uint32_t col = part * kLanes * (16 / sizeof(T));
+        const bool in = lane_col + col < a.head && i * kRowsAt + lane_row < have;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to_at + static_cast<uint32_t>((i * kRowsAt * P + col) * sizeof(T))), "l"(in ? from_at + col : kb), "r"(in ? 16u : 0u) : "memory");
+      }
+      from_at += stride;
+    }
+  };
   auto load_step = [&](uint32_t i) {
     if (i < steps) {
-      T *at = mine + i % kStages * (2 * BN * P);
-      load_rows<T, kD, BN, 32>(at, kb, a.k_ld, 1, first + i * kRound, to, a.head, wide & kWideK, lane);
-      load_rows<T, kD, BN, 32>(at + BN * P, vb, a.v_ld, 1, first + i * kRound, to, a.head, wide & kWideV, lane);
+      const uint32_t key0 = first + i * kRound, have = min(to - key0, static_cast<uint32_t>(BN));
+      if (apart) {
+        T *at = mine + load_at * (2 * BN * P);
+        load_rows<T, kD, BN, 32>(at, kb, a.k_ld, 1, key0, to, a.head, false, lane);
+        load_rows<T, kD, BN, 32>(at + BN * P, vb, a.v_ld, 1, key0, to, a.head, false, lane);
+      } else {
+        const uint32_t to_at = lane_to + load_at * static_cast<uint32_t>(2 * BN * P * sizeof(T));
+        copy_rows(to_at, k_from, k_rows, have);
+        copy_rows(to_at + static_cast<uint32_t>(BN * P * sizeof(T)), v_from, v_rows, have);
+        k_from += kRound * a.k_ld, v_from += kRound * a.v_ld;
+      }
+      if (++load_at == kStages) load_at = 0;
     }
     copies_commit();
   };
   load_rows<T, kD, 16, kThreads>(sq, qb, a.q_ld, a.group, row0, rows, a.head, wide & kWideQ);
   copies_commit();
-  load_step(0);
-  load_step(1);
-  copies_wait<2>();
-  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i + 1 < kStages; ++i) load_step(i);
+  copies_wait<kStages - 1>();
+  __syncthreads();          // queries
+  uint32_t qf[kHalf ? kD / 16 : 1][4];
+  if constexpr (kHalf) {
+#pragma unroll
+    for (int kk = 0; kk < kD / 16; ++kk) ldsm4(qf[kk], smem_at(sq) + ((lane & 15u) * P + (lane >> 4) * 8u + kk * 16) * 2u);
+  } else {
+    for (uint32_t i = threadIdx.x; i < 16 * P; i += kThreads) {
+      uint32_t hi, lo = 0;
+      split<kPass>(sq[i], hi, lo);
+      sq[i] = __uint_as_float(hi), sq[16 * P + i] = __uint_as_float(lo);
+    }
+    __syncthreads();
+  }
 
+  // the last key that each of this lane's two rows sees, and the first step in which one of the warp's rows does not see all
   uint32_t row[2];
-  long long last[2];
+  int last[2];
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     row[r] = row0 + g + r * 8;
-    last[r] = row[r] >= rows ? -1 : (a.causal ? static_cast<long long>(row[r] / a.group) + shift : static_cast<long long>(q.lk) - 1);
-    last[r] = min(last[r], static_cast<long long>(to) - 1);
+    long long see = row[r] >= rows ? static_cast<long long>(to) - 1 : (a.causal ? static_cast<long long>(row[r] / a.group) + shift : static_cast<long long>(q.lk) - 1);
+    see = min(see, static_cast<long long>(to) - 1);
+    last[r] = static_cast<int>(max(see, -1ll));
   }
+  const int all = __reduce_min_sync(0xffffffffu, min(last[0], last[1])) + 1;   // keys that every row sees
   float acc[kD / 8][4];
 #pragma unroll
   for (int n = 0; n < kD / 8; ++n)
@@ -94,29 +217,48 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
     for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
   const float to2 = a.scale * kLog2e;
 
-  for (uint32_t i = 0; i < steps; ++i) {
-    copies_wait<1>();
-    __syncwarp();          // every lane's copies of this step are in, and the step before is read
-    load_step(i + 2);
-    const T *sk = mine + i % kStages * (2 * BN * P);
+  uint32_t at = 0;
+  int key0 = static_cast<int>(first);
+  for (uint32_t i = 0; i < steps; ++i, key0 += kRound) {
+    copies_wait<kStages - 2>();
+    __syncwarp();          // every lane's copies of this step are in, and the slot of the step before is read
+    load_step(i + kStages - 1);
+    const T *sk = mine + at * (2 * BN * P);
     float s[NT][4];
-    product_abt<kD, NT, kPass>(s, sq, sk);
-    const uint32_t key0 = first + i * kRound;
-    float top[2] = {-INFINITY, -INFINITY}, keep[2];
+    if constexpr (kHalf) scores<kD, NT>(s, qf, sk);
+    else scores<kD, NT, kPass>(s, sq, sq + 16 * P, sk);
+    if (key0 + BN > all) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (key0 + n * 8 + static_cast<int>(2 * t) + (e & 1) > last[e >> 1]) s[n][e] = -INFINITY;
+          else s[n][e] *= to2;
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] *= to2;
+    }
+    float top[2] = {m[0], m[1]};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool seen = static_cast<long long>(key0 + n * 8 + 2 * t + (e & 1)) <= last[e >> 1];
-        s[n][e] = seen ? s[n][e] * to2 : -INFINITY;
-        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+      for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+    top[0] = quad_max(top[0]), top[1] = quad_max(top[1]);
+    if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float keep = top[r] == m[r] ? 1.f : exp2_of<T>(m[r] - top[r]);
+        m[r] = top[r];
+        l[r] *= keep;
+#pragma unroll
+        for (int n = 0; n < kD / 8; ++n) acc[n][2 * r] *= keep, acc[n][2 * r + 1] *= keep;
       }
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float now = fmaxf(m[r], quad_max(top[r])), base = now == -INFINITY ? 0.f : now;
-      keep[r] = exp2_of<T>(m[r] - base);
-      m[r] = now;
-      l[r] *= keep[r];
+      const float base = m[r] == -INFINITY ? 0.f : m[r];   // nothing seen yet: every p below is exp2(-inf)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -126,12 +268,13 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
           l[r] += p;
         }
     }
-    product_py<kD, kD, NT, kPass>(acc, s, sk + BN * P, 0, keep[0], keep[1]);
+    add_values<kD, kPass>(acc, s, sk + BN * P);
+    if (++at == kStages) at = 0;
   }
   copies_wait<0>();
 
   // ---- the warps' parts ----
-  float *part = reinterpret_cast<float *>(ring);
+  float *part = reinterpret_cast<float *>(ring_at);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] = quad_sum(l[r]);
@@ -229,7 +372,7 @@ int launch_tokens(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
   // Two blocks for every SM, and no more than 1024 keys for one, so that sequences of different lengths even out; two rounds of
   // the warps at least.
   const unsigned long long sms = static_cast<unsigned long long>(ctx->sm_count);
-  const unsigned long long want = std::max((2 * sms + items - 1) / items, (a.max_k + 1023ull) / 1024ull);
+  const unsigned long long want = std::max((2 * sms + items - 1) / items, (a.max_k + 4095ull) / 4096ull);
   uint32_t splits = 1;
   while (splits < kMaxSplits && splits < want && a.max_k / (2 * splits) >= 2 * kWarps * kStep<T>) splits *= 2;
   if (items * splits > 0x7fffffffull) return B200_ERR_TOO_LARGE;

@@ -4,19 +4,22 @@
 //   norm_rotary   n = x r, r = 1 / sqrt(mean(x^2) + eps);  y = turned (n gain)
 //   backward      g = gy turned back (t -> -t);  ggain += sum g n;  gx += r (g gain - n mean(g gain n))
 //
-// Bound by memory: one read and one write of every element (three with a backward norm).  A group of lanes
-// (a power of two) holds one head of one token in registers, so the norm's sums are a few shuffles and nothing is
-// read twice.  A lane's unit is the two vectors that turn with one another: in the HALVES layout they lie rot/2
+// Bound by memory, one read and one write of every element (three with a backward norm), if the instructions beside
+// it are few.  A group of lanes (a power of two) holds one head of one token in registers, so the norm's sums are a few shuffles and
+// nothing is read twice.  A lane's unit is the two vectors that turn with one another: in the HALVES layout they lie rot/2
 // apart, in the PAIRS layout side by side.
 //
-// The cosines depend on the token alone.  A block takes a tile of tokens, forms their angles once, in shared memory,
-// and every head reads them from there: with each head forming its own, 40 heads of 128 would cost 2.6 million
-// 64-bit products and sines per 1024 tokens instead of 65 thousand.  An angle is formed in turns and reduced in 64 bits,
-// so position 1000000 has the same error (2^-26 of a turn) as position 0; its sine and cosine are 32-bit.
+// The cosines depend on the token alone.  A block takes a tile of tokens and forms their angles once, in shared memory: with each head
+// forming its own, 40 heads of 128 would cost 2.6 million 64-bit products and sines per 1024 tokens instead of 65 thousand.  A
+// group stays with one token and goes over its heads, with the token's cosines and the gain in registers; arithmetic is on pairs of floats.
+// (A group that took any row, and read cosines and gain for it, spent two to three times the instructions: 71 us forward, 91 us with norms,
+// 266 us for their gradient, where this takes 62, 84 and 116; 16384 tokens of 40 heads of 128 halves.)
+// An angle is formed in turns and reduced in 64 bits, so position 1000000 has the same error (2^-26 of a turn) as position
+// 0; its sine and cosine are 32-bit.
 //
-// Gradients of gains are sums over every token and head.  Each thread keeps its elements' sums in registers over all
-// the rows its block takes, a block writes one partial row and a second kernel adds the rows in order: no atomics, the
-// same bits every run.
+// With norms a block takes the heads of one gain only.  Gradients of gains are sums over every token and head: a thread keeps its
+// elements' sums in registers over all that its block takes, a block writes one partial row and a second kernel adds the
+// rows in order: no atomics, the same bits every run.
 #include <algorithm>
 #include <cmath>
 
@@ -29,19 +32,22 @@ namespace {
 constexpr unsigned kThreads = 256;
 constexpr unsigned kWarps = kThreads / 32;
 constexpr uint32_t kMaxHead = 256;
-constexpr uint32_t kMaxTile = 16;          // tokens per block
-constexpr uint32_t kMaxPartials = B200_NORM_ROTARY_SCRATCH / (2 * kMaxHead);
+constexpr uint32_t kHeadsEach = 8;
+constexpr uint32_t kSumBlocks = 3;         // blocks per SM that keep sums
+constexpr uint32_t kMaxPartials = B200_NORM_ROTARY_SCRATCH / kMaxHead;
 
 struct RotaryArgs {
   const void *x, *g;        // forward: x; backward: g = gy, and x where there is a norm
   void *y;                  // y or gx
   const void *gain_q, *gain_k;
-  float *partial;           // [block][q, k][head], or null
+  float *partial;           // [block][head], or null
   const double *freqs;
   const uint32_t *positions;
   u64 x_ld, g_ld, y_ld;
   uint32_t head, heads, heads_q, tokens, rot;
-  uint32_t units, lanes_log2, tile;   // units of a head; lanes of a group; tokens of a tile
+  uint32_t units, lanes_log2;         // units of a head; lanes of a group
+  // Blocks 0 .. blocks_q - 1 take the first heads_q heads, the others the rest.  Of a block's groups 2^split_log2 share a token.
+  uint32_t blocks_q, split_q_log2, split_k_log2;
   float amplitude, eps;
   int accumulate;
 };
@@ -74,86 +80,190 @@ __device__ __forceinline__ void unit_at(uint32_t u, uint32_t rot, uint32_t &c0, 
   c1 = c0 + V;
 }
 
-// Elements 0 .. V-1 of w are the first vector, V .. 2V-1 the second.  `tab`: this token's row of the table.
-template <int V, int kLayout>
-__device__ __forceinline__ void turn(float (&w)[2 * V], uint32_t u, uint32_t rot, const float2 *tab, uint32_t pitch) {
+// Pairs of floats.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// V floats, as pairs where there are two.
+template <int V>
+struct Lane {
+  f32x2 p[V > 1 ? V / 2 : 1];
+  __device__ __forceinline__ void put(int j, float v) {
+    float a, b;
+    unpair(p[j / 2], a, b);
+    p[j / 2] = (j & 1) ? pair_of(a, v) : pair_of(v, b);
+  }
+  __device__ __forceinline__ float get(int j) const {
+    float a, b;
+    unpair(p[j / 2], a, b);
+    return (j & 1) ? b : a;
+  }
+};
+template <int V> __device__ __forceinline__ Lane<V> operator*(const Lane<V> &x, const Lane<V> &y) {
+  Lane<V> z;
+#pragma unroll
+  for (int i = 0; i < (V > 1 ? V / 2 : 1); ++i) z.p[i] = mul2(x.p[i], y.p[i]);
+  return z;
+}
+template <int V> __device__ __forceinline__ Lane<V> fma(const Lane<V> &x, const Lane<V> &y, const Lane<V> &c) {
+  Lane<V> z;
+#pragma unroll
+  for (int i = 0; i < (V > 1 ? V / 2 : 1); ++i) z.p[i] = fma2(x.p[i], y.p[i], c.p[i]);
+  return z;
+}
+template <int V> __device__ __forceinline__ Lane<V> all_of(float v) {
+  Lane<V> z;
+#pragma unroll
+  for (int i = 0; i < (V > 1 ? V / 2 : 1); ++i) z.p[i] = pair_of(v, V > 1 ? v : 0.f);
+  return z;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <int V> __device__ __forceinline__ float sum_of(const Lane<V> &x) {
+  f32x2 s[V > 1 ? V / 2 : 1];
+#pragma unroll
+  for (int i = 0; i < (V > 1 ? V / 2 : 1); ++i) s[i] = x.p[i];
+#pragma unroll
+  for (int n = V / 4; n > 0; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) s[i] = add2(s[i], s[i + n]);
+  float a, b;
+  unpair(s[0], a, b);
+  return V > 1 ? a + b : a;
+}
+
+// A unit's pairs: a[j] turns with b[j].
+template <int V>
+struct Unit {
+  Lane<V> a, b;
+};
+
+// A unit as it lies in memory.
+template <typename T, int V>
+struct Raw {
+  Pack<T, V> first, second;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_raw(Raw<T, V> &raw, const T *p, uint32_t c0, uint32_t c1, uint32_t head) {
+  if (c0 < head) raw.first = *reinterpret_cast<const Pack<T, V> *>(p + c0);
+  if (c1 < head) raw.second = *reinterpret_cast<const Pack<T, V> *>(p + c1);
+}
+// What there is none of counts as zero.
+template <typename T, int V, int kLayout>
+__device__ __forceinline__ Unit<V> unit_of(const Raw<T, V> &raw, bool has0, bool has1) {
+  Unit<V> u;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int ia = kLayout == B200_ROTARY_HALVES ? j : 2 * j, ib = kLayout == B200_ROTARY_HALVES ? j + V : 2 * j + 1;
-    if (2 * (u * V + j) < rot) {
-      const float2 cs = tab[j * pitch + u];
-      const float a = w[ia], b = w[ib];
-      w[ia] = a * cs.x - b * cs.y;
-      w[ib] = b * cs.x + a * cs.y;
+    // element e of the two vectors' 2 V
+    const int ea = kLayout == B200_ROTARY_HALVES ? j : 2 * j, eb = kLayout == B200_ROTARY_HALVES ? j + V : 2 * j + 1;
+    const float x = ea < V ? (has0 ? to_float(raw.first.v[ea < V ? ea : 0]) : 0.f) : (has1 ? to_float(raw.second.v[ea < V ? 0 : ea - V]) : 0.f);
+    const float y = eb < V ? (has0 ? to_float(raw.first.v[eb < V ? eb : 0]) : 0.f) : (has1 ? to_float(raw.second.v[eb < V ? 0 : eb - V]) : 0.f);
+    u.a.put(j, x), u.b.put(j, y);
+  }
+  return u;
+}
+template <typename T, int V, int kLayout>
+__device__ __forceinline__ void store_unit(const Unit<V> &u, T *p, uint32_t c0, uint32_t c1, uint32_t head) {
+  Pack<T, V> first, second;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if constexpr (kLayout == B200_ROTARY_HALVES) {
+      first.v[e] = from_float<T>(u.a.get(e)), second.v[e] = from_float<T>(u.b.get(e));
+    } else {
+      first.v[e] = from_float<T>((e & 1) ? u.b.get(e / 2) : u.a.get(e / 2));
+      second.v[e] = from_float<T>(((e + V) & 1) ? u.b.get((e + V) / 2) : u.a.get((e + V) / 2));
     }
   }
+  if (c0 < head) *reinterpret_cast<Pack<T, V> *>(p + c0) = first;
+  if (c1 < head) *reinterpret_cast<Pack<T, V> *>(p + c1) = second;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void load_unit(float (&w)[2 * V], const T *p, uint32_t c0, uint32_t c1, uint32_t head) {
-  Pack<T, V> a, b;
-  const bool has0 = c0 < head, has1 = c1 < head;
-  if (has0) a = *reinterpret_cast<const Pack<T, V> *>(p + c0);
-  if (has1) b = *reinterpret_cast<const Pack<T, V> *>(p + c1);
+// The group's sums of both, side by side.
+template <int kLog2>
+__device__ __forceinline__ void sums_over(float &v, float &w) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    w[j] = has0 ? to_float(a.v[j]) : 0.f;
-    w[V + j] = has1 ? to_float(b.v[j]) : 0.f;
+  for (int o = 1; o < 1 << kLog2; o <<= 1) {
+    const float x = __shfl_xor_sync(0xffffffffu, v, o), y = __shfl_xor_sync(0xffffffffu, w, o);
+    v += x, w += y;
   }
 }
-
-template <typename T, int V>
-__device__ __forceinline__ void store_unit(const float (&w)[2 * V], T *p, uint32_t c0, uint32_t c1, uint32_t head) {
-  Pack<T, V> a, b;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    a.v[j] = from_float<T>(w[j]);
-    b.v[j] = from_float<T>(w[V + j]);
+__device__ __forceinline__ void group_sums(float &v, float &w, uint32_t lanes_log2) {
+  switch (lanes_log2) {
+    case 0: break;
+    case 1: sums_over<1>(v, w); break;
+    case 2: sums_over<2>(v, w); break;
+    case 3: sums_over<3>(v, w); break;
+    case 4: sums_over<4>(v, w); break;
+    default: sums_over<5>(v, w); break;
   }
-  if (c0 < head) *reinterpret_cast<Pack<T, V> *>(p + c0) = a;
-  if (c1 < head) *reinterpret_cast<Pack<T, V> *>(p + c1) = b;
-}
-
-__device__ __forceinline__ float group_sum(float v, uint32_t lanes) {
-  for (uint32_t o = 1; o < lanes; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
 }
 
 // kUnits: units per lane (heads are at most 256 elements, so single elements need four, pairs two).
-// kRows: rows a lane has in flight.  One would leave HBM waiting: 16 Ki tokens of 40 heads of 128 halves.
+template <int V> constexpr int kUnitsOf = V >= 4 ? 1 : (V == 2 ? 2 : 4);
+
 template <typename T, int V, int kLayout, bool kNorm, bool kBack>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   pdl_enter();
-  constexpr int kUnits = V >= 4 ? 1 : (V == 2 ? 2 : 4);
-  constexpr int kRows = kUnits == 1 && !(kNorm && kBack) ? 2 : 1;
-  extern __shared__ float2 s_tab[];                                  // [tile][V][pitch]
-  __shared__ float s_gain[kNorm ? 2 * kMaxHead : 1];
-  __shared__ float s_sums[kNorm && kBack ? kWarps * 2 * kMaxHead : 1];
+  constexpr int kUnits = kUnitsOf<V>;
+  constexpr bool kSums = kNorm && kBack;
+  // Where sums are kept, registers leave room for three blocks on an SM, whose loads alone do not fill the memory's latency: the next row
+  // is fetched into shared memory, where every thread has slots of its own.  (Into registers: two blocks, 199 us instead of 116.)
+  constexpr bool kStaged = kSums && kUnits == 1 && V * sizeof(T) >= 8;
+  constexpr uint32_t kStages = 2;   // (three or four: the same time)
+  extern __shared__ float2 s_tab[];                                  // [token][V][pitch]
+  __shared__ float s_sums[kSums ? kWarps * kMaxHead : 1];
+  __shared__ __align__(16) Pack<T, V> s_slots[kStaged ? kStages * 4 : 1][kThreads];
 
-  const uint32_t lanes = 1u << a.lanes_log2, lane = threadIdx.x & (lanes - 1), first_row = threadIdx.x >> a.lanes_log2;
-  const uint32_t row_step = kThreads >> a.lanes_log2;
+  const bool second = blockIdx.x >= a.blocks_q;
+  const uint32_t block = second ? blockIdx.x - a.blocks_q : blockIdx.x, blocks = second ? gridDim.x - a.blocks_q : a.blocks_q;
+  const uint32_t head0 = second ? a.heads_q : 0u, heads = second ? a.heads - a.heads_q : a.heads_q;
+  const uint32_t split_log2 = second ? a.split_k_log2 : a.split_q_log2, split = 1u << split_log2;
+  const uint32_t lanes = 1u << a.lanes_log2, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> a.lanes_log2;
+  const uint32_t tile_tokens = (kThreads >> a.lanes_log2) >> split_log2, tiles = (a.tokens + tile_tokens - 1) / tile_tokens;
+  const uint32_t my_tok = group >> split_log2, my_head = group & (split - 1), turns_of_heads = (heads + split - 1) >> split_log2;
   const uint32_t pairs = a.rot / 2, pitch = (pairs + V - 1) / V, tab_size = V * pitch;
-  const uint32_t tiles = (a.tokens + a.tile - 1) / a.tile;
+
+  uint32_t c0[kUnits], c1[kUnits];
+  bool turned[kUnits];
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    unit_at<V, kLayout>(lane + k * lanes, a.rot, c0[k], c1[k]);
+    turned[k] = 2 * (lane + k * lanes) * V < a.rot;
+  }
+  Unit<V> gain[kNorm ? kUnits : 1], sums[kSums ? kUnits : 1];
   if constexpr (kNorm) {
-    for (uint32_t i = threadIdx.x; i < 2 * a.head; i += kThreads) {
-      const bool k = i >= a.head;
-      const T *gain = static_cast<const T *>(k ? a.gain_k : a.gain_q);
-      s_gain[i] = gain ? to_float(gain[k ? i - a.head : i]) : 0.f;
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      Raw<T, V> raw;
+      load_raw(raw, static_cast<const T *>(second ? a.gain_k : a.gain_q), c0[k], c1[k], a.head);
+      gain[k] = unit_of<T, V, kLayout>(raw, c0[k] < a.head, c1[k] < a.head);
+      if constexpr (kSums) sums[k].a = sums[k].b = all_of<V>(0.f);
     }
   }
-  float sums[kNorm && kBack ? 2 : 1][kUnits][2 * V];
-  if constexpr (kNorm && kBack) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int k = 0; k < kUnits; ++k)
-#pragma unroll
-        for (int j = 0; j < 2 * V; ++j) sums[s][k][j] = 0.f;
-  }
+  const float per_head = 1.f / static_cast<float>(a.head);
 
-  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const uint32_t t0 = tile * a.tile, nt = min(a.tile, a.tokens - t0);
-    __syncthreads();   // the table's last readers are done
+  for (uint32_t tile = block; tile < tiles; tile += blocks) {
+    const uint32_t t0 = tile * tile_tokens, nt = min(tile_tokens, a.tokens - t0);
+    if (tile != block) __syncthreads();   // the table's last readers are done
     for (uint32_t i = threadIdx.x; i < nt * pairs; i += kThreads) {
       const uint32_t t = i / pairs, p = i - t * pairs;
       const double pos = a.positions ? static_cast<double>(a.positions[t0 + t]) : static_cast<double>(t0 + t);
@@ -162,135 +272,161 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
       sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
       s_tab[t * tab_size + (p % V) * pitch + p / V] = make_float2(a.amplitude * cs, a.amplitude * (kBack ? -sn : sn));
     }
-    __syncthreads();
-    const uint32_t rows = nt * a.heads, rounds = (rows + row_step - 1) / row_step;   // the same for every lane: shuffles below
-    for (uint32_t round = 0; round < rounds; round += kRows) {
-      float w[kRows][kUnits][2 * V], gw[kNorm && kBack ? kRows : 1][kUnits][2 * V];
-      uint32_t tok[kRows], h[kRows];
-      bool live[kRows];
+    if constexpr (kStaged) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const bool live = my_tok < nt;
+    const u64 t = t0 + my_tok, at = static_cast<u64>(head0 + my_head) * a.head, step = static_cast<u64>(a.head) << split_log2;
+    const T *x = static_cast<const T *>(kBack && !kNorm ? a.g : a.x) + t * (kBack && !kNorm ? a.g_ld : a.x_ld) + at;
+    const T *g = static_cast<const T *>(a.g) + t * a.g_ld + at;
+    T *out = static_cast<T *>(a.y) + t * a.y_ld + at;
+    Raw<T, V> raw[kUnits], raw_g[kSums ? kUnits : 1];
+    auto fetch = [&](uint32_t i) {
+      const uint32_t head = live && my_head + (i << split_log2) < heads ? a.head : 0u;
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const uint32_t row = first_row + (round + r) * row_step;
-        live[r] = row < rows;
-        tok[r] = live[r] ? row / a.heads : 0u;
-        h[r] = live[r] ? row - tok[r] * a.heads : 0u;
-#pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-          uint32_t c0, c1;
-          unit_at<V, kLayout>(lane + k * lanes, a.rot, c0, c1);
-          const uint32_t head = live[r] ? a.head : 0u;
-          const u64 t = t0 + tok[r], at = static_cast<u64>(h[r]) * a.head;
-          load_unit<T, V>(w[r][k], static_cast<const T *>(kBack && !kNorm ? a.g : a.x) + t * (kBack && !kNorm ? a.g_ld : a.x_ld) + at, c0, c1, head);
-          if constexpr (kNorm && kBack) load_unit<T, V>(gw[r][k], static_cast<const T *>(a.g) + t * a.g_ld + at, c0, c1, head);
-        }
+      for (int k = 0; k < kUnits; ++k) {
+        load_raw(raw[k], x, c0[k], c1[k], head);
+        if constexpr (kSums) load_raw(raw_g[k], g, c0[k], c1[k], head);
       }
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const float2 *tab = s_tab + tok[r] * tab_size;
-        if constexpr (kNorm) {
-          float ss = 0.f;
-#pragma unroll
-          for (int k = 0; k < kUnits; ++k)
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) ss += w[r][k][j] * w[r][k][j];
-          ss = group_sum(ss, lanes);
-          const float rs = 1.f / sqrtf(ss / static_cast<float>(a.head) + a.eps);
-          const uint32_t is_k = h[r] >= a.heads_q ? 1u : 0u;
-          const float *gain = s_gain + is_k * a.head;
-          if constexpr (!kBack) {
-#pragma unroll
-            for (int k = 0; k < kUnits; ++k) {
-              uint32_t c0, c1;
-              unit_at<V, kLayout>(lane + k * lanes, a.rot, c0, c1);
-#pragma unroll
-              for (int j = 0; j < V; ++j) {
-                w[r][k][j] *= rs * (c0 < a.head ? gain[c0 + j] : 0.f);
-                w[r][k][V + j] *= rs * (c1 < a.head ? gain[c1 + j] : 0.f);
-              }
-            }
-          } else {
-            float dot = 0.f;
-#pragma unroll
-            for (int k = 0; k < kUnits; ++k) {
-              uint32_t c0, c1;
-              unit_at<V, kLayout>(lane + k * lanes, a.rot, c0, c1);
-              turn<V, kLayout>(gw[r][k], lane + k * lanes, a.rot, tab, pitch);
-#pragma unroll
-              for (int j = 0; j < 2 * V; ++j) {
-                w[r][k][j] *= rs;                                        // n
-                const float gn = gw[r][k][j] * w[r][k][j];
-                if (live[r]) sums[0][k][j] += is_k ? 0.f : gn, sums[1][k][j] += is_k ? gn : 0.f;
-                const uint32_t c = j < V ? c0 : c1;
-                gw[r][k][j] *= c < a.head ? gain[c + (j < V ? j : j - V)] : 0.f;
-                dot += gw[r][k][j] * w[r][k][j];
-              }
-            }
-            dot = group_sum(dot, lanes) / static_cast<float>(a.head);
-#pragma unroll
-            for (int k = 0; k < kUnits; ++k)
-#pragma unroll
-              for (int j = 0; j < 2 * V; ++j) w[r][k][j] = rs * (gw[r][k][j] - w[r][k][j] * dot);
-          }
+      x += step;
+      if constexpr (kSums) g += step;
+    };
+    // the same into a stage's slots
+    auto stage = [&](uint32_t i) {
+      if constexpr (kStaged) {
+        if (live && i < turns_of_heads && my_head + (i << split_log2) < heads) {
+          auto copy = [&](uint32_t slot, const T *from) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&s_slots[(i % kStages) * 4 + slot][threadIdx.x]))),
+                         "l"(from), "n"(static_cast<int>(V * sizeof(T))) : "memory");
+          };
+          if (c0[0] < a.head) copy(0, x + c0[0]), copy(2, g + c0[0]);
+          if (c1[0] < a.head) copy(1, x + c1[0]), copy(3, g + c1[0]);
         }
-        if (!live[r]) continue;
-        T *out = static_cast<T *>(a.y) + static_cast<u64>(t0 + tok[r]) * a.y_ld + static_cast<u64>(h[r]) * a.head;
+        x += step, g += step;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+    };
+    if constexpr (kStaged) {
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-          uint32_t c0, c1;
-          unit_at<V, kLayout>(lane + k * lanes, a.rot, c0, c1);
-          if constexpr (!(kNorm && kBack)) turn<V, kLayout>(w[r][k], lane + k * lanes, a.rot, tab, pitch);
-          if constexpr (kBack) {
-            if (a.accumulate) {
-              float old[2 * V];
-              load_unit<T, V>(old, out, c0, c1, a.head);
+      for (uint32_t i = 0; i + 1 < kStages; ++i) stage(i);
+    } else {
+      fetch(0);
+    }
+    __syncthreads();
+    Unit<V> cs[kUnits];   // a: cosine, b: sine
 #pragma unroll
-              for (int j = 0; j < 2 * V; ++j) w[r][k][j] += old[j];
-            }
-          }
-          store_unit<T, V>(w[r][k], out, c0, c1, a.head);
+    for (int k = 0; k < kUnits; ++k) {
+      cs[k].a = all_of<V>(1.f), cs[k].b = all_of<V>(0.f);
+      if (live && turned[k]) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float2 v = s_tab[my_tok * tab_size + j * pitch + lane + k * lanes];
+          cs[k].a.put(j, v.x), cs[k].b.put(j, v.y);
         }
       }
     }
+    auto turn = [&](Unit<V> &u, int k) {
+      if (!turned[k]) return;
+      const Lane<V> minus = all_of<V>(-1.f) * cs[k].b, a1 = fma(u.b, minus, u.a * cs[k].a);
+      u.b = fma(u.a, cs[k].b, u.b * cs[k].a);
+      u.a = a1;
+    };
+    for (uint32_t i = 0; i < turns_of_heads; ++i) {
+      if constexpr (kStaged) {
+        stage(i + kStages - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        const Pack<T, V> (*slots)[kThreads] = s_slots + (i % kStages) * 4;
+        raw[0].first = slots[0][threadIdx.x], raw[0].second = slots[1][threadIdx.x];
+        raw_g[0].first = slots[2][threadIdx.x], raw_g[0].second = slots[3][threadIdx.x];
+      } else if (i > 0) {
+        fetch(i);
+      }
+      const bool here = live && my_head + (i << split_log2) < heads;
+      Unit<V> w[kUnits], gw[kSums ? kUnits : 1];
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+        w[k] = unit_of<T, V, kLayout>(raw[k], here && c0[k] < a.head, here && c1[k] < a.head);
+        if constexpr (kSums) gw[k] = unit_of<T, V, kLayout>(raw_g[k], here && c0[k] < a.head, here && c1[k] < a.head);
+      }
+      if constexpr (kNorm) {
+        Lane<V> sq = all_of<V>(0.f), dots = all_of<V>(0.f);
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+          sq = fma(w[k].b, w[k].b, fma(w[k].a, w[k].a, sq));
+          if constexpr (kBack) {
+            turn(gw[k], k);
+            dots = fma(gw[k].b * gain[k].b, w[k].b, fma(gw[k].a * gain[k].a, w[k].a, dots));
+          }
+        }
+        float ss = sum_of(sq), dot = kBack ? sum_of(dots) : 0.f;
+        group_sums(ss, dot, a.lanes_log2);
+        const float rs = rsqrtf(ss * per_head + a.eps);
+        const Lane<V> rs_all = all_of<V>(rs);
+        if constexpr (!kBack) {
+#pragma unroll
+          for (int k = 0; k < kUnits; ++k) w[k].a = w[k].a * (rs_all * gain[k].a), w[k].b = w[k].b * (rs_all * gain[k].b);
+        } else {
+          const Lane<V> minus_dot = all_of<V>(-per_head * rs * dot);
+#pragma unroll
+          for (int k = 0; k < kUnits; ++k) {
+            w[k].a = w[k].a * rs_all, w[k].b = w[k].b * rs_all;          // n; zero where there is no row
+            sums[k].a = fma(gw[k].a, w[k].a, sums[k].a), sums[k].b = fma(gw[k].b, w[k].b, sums[k].b);
+            w[k].a = rs_all * fma(w[k].a, minus_dot, gw[k].a * gain[k].a), w[k].b = rs_all * fma(w[k].b, minus_dot, gw[k].b * gain[k].b);
+          }
+        }
+      }
+      if (here) {
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+          if constexpr (!kSums) turn(w[k], k);
+          if constexpr (kBack) {
+            if (a.accumulate) {
+              Raw<T, V> raw_old;
+              load_raw(raw_old, static_cast<const T *>(out), c0[k], c1[k], a.head);
+              const Unit<V> old = unit_of<T, V, kLayout>(raw_old, c0[k] < a.head, c1[k] < a.head);
+              const Lane<V> one = all_of<V>(1.f);
+              w[k].a = fma(old.a, one, w[k].a), w[k].b = fma(old.b, one, w[k].b);
+            }
+          }
+          store_unit<T, V, kLayout>(w[k], out, c0[k], c1[k], a.head);
+        }
+      }
+      out += step;
+    }
   }
 
-  if constexpr (kNorm && kBack) {
+  if constexpr (kSums) {
     if (!a.partial) return;
     const uint32_t warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int k = 0; k < kUnits; ++k)
 #pragma unroll
-      for (int k = 0; k < kUnits; ++k) {
-        uint32_t c0, c1;
-        unit_at<V, kLayout>(lane + k * lanes, a.rot, c0, c1);
-#pragma unroll
-        for (int j = 0; j < 2 * V; ++j) {
-          float v = sums[s][k][j];
-          for (uint32_t o = lanes; o < 32u; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          const uint32_t c = (j < V ? c0 : c1), at = c + (j < V ? j : j - V);
-          if ((threadIdx.x & 31u) < lanes && c < a.head) s_sums[(warp * 2 + s) * kMaxHead + at] = v;
-        }
+      for (int e = 0; e < 2 * V; ++e) {
+        const bool is_b = kLayout == B200_ROTARY_HALVES ? e >= V : (e & 1);
+        float v = is_b ? sums[k].b.get(kLayout == B200_ROTARY_HALVES ? e - V : e / 2) : sums[k].a.get(kLayout == B200_ROTARY_HALVES ? e : e / 2);
+        for (uint32_t o = lanes; o < 32u; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        const uint32_t c = e < V ? c0[k] : c1[k], at = c + (e < V ? e : e - V);
+        if ((threadIdx.x & 31u) < lanes && c < a.head) s_sums[warp * kMaxHead + at] = v;
       }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 2 * a.head; i += kThreads) {
-      const uint32_t s = i >= a.head ? 1u : 0u, at = i - s * a.head;
+    for (uint32_t i = threadIdx.x; i < a.head; i += kThreads) {
       float v = 0.f;
 #pragma unroll
-      for (unsigned wp = 0; wp < kWarps; ++wp) v += s_sums[(wp * 2 + s) * kMaxHead + at];
-      a.partial[(static_cast<u64>(blockIdx.x) * 2 + s) * a.head + at] = v;
+      for (unsigned wp = 0; wp < kWarps; ++wp) v += s_sums[wp * kMaxHead + i];
+      a.partial[static_cast<u64>(blockIdx.x) * a.head + i] = v;
     }
   }
 }
 
 // ggain = (accumulate ? ggain : 0) + the blocks' rows, added in order by 32 lanes of threads and then those in order.
 template <typename T>
-__global__ void __launch_bounds__(1024) gain_sums_kernel(const float *partial, uint32_t rows, uint32_t head, T *gq, T *gk, int accumulate) {
+__global__ void __launch_bounds__(1024) gain_sums_kernel(const float *partial, uint32_t rows_q, uint32_t rows, uint32_t head, T *gq, T *gk, int accumulate) {
   pdl_enter();
   __shared__ float s[32][33];
   const uint32_t col = blockIdx.x * 32 + threadIdx.x;
   float v = 0.f;
   if (col < 2 * head)
 #pragma unroll 4
-    for (uint32_t r = threadIdx.y; r < rows; r += 32) v += partial[static_cast<u64>(r) * 2 * head + col];
+    for (uint32_t r = threadIdx.y + (col < head ? 0u : rows_q); r < (col < head ? rows_q : rows); r += 32)
+      v += partial[static_cast<u64>(r) * head + (col < head ? col : col - head)];
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.y != 0 || col >= 2 * head) return;
@@ -305,49 +441,67 @@ __global__ void __launch_bounds__(1024) gain_sums_kernel(const float *partial, u
 // The widest vectors that every address and extent allows.
 template <typename T>
 uint32_t vector_width(const RotaryArgs &a, int layout, int back, int norm) {
-  uint32_t v = 16 / sizeof(T);
+  uint32_t v = norm ? 4 : 16 / sizeof(T);   // (with norms eight halves a lane take so many registers that four are faster)
   auto fits = [&](uint32_t n) {
     auto ok = [&](const void *p, u64 ld) { return !p || (reinterpret_cast<uintptr_t>(p) % (n * sizeof(T)) == 0 && ld % n == 0); };
     if (!ok(a.y, a.y_ld) || ((!back || norm) && !ok(a.x, a.x_ld)) || (back && !ok(a.g, a.g_ld))) return false;
-    return a.head % n == 0 && (layout == B200_ROTARY_PAIRS || (a.rot / 2) % n == 0);
+    return a.head % n == 0 && (layout == B200_ROTARY_PAIRS ? a.rot % (2 * n) == 0 : (a.rot / 2) % n == 0);
   };
   while (v > 1 && !fits(v)) v /= 2;
   return v;
 }
 
 template <typename T, int V, int kLayout, bool kNorm, bool kBack>
-int launch_rotary(b200_ctx *ctx, cudaStream_t s, RotaryArgs a) {
+int launch_rotary(b200_ctx *ctx, cudaStream_t s, RotaryArgs a, uint32_t *rows_q) {
   const uint32_t turned = a.rot / 2 / V;
   a.units = kLayout == B200_ROTARY_HALVES ? turned + ((a.head - a.rot) / V + 1) / 2 : (a.head / V + 1) / 2;
-  constexpr int kUnits = V >= 4 ? 1 : (V == 2 ? 2 : 4);
   a.lanes_log2 = 0;
-  while ((kUnits << a.lanes_log2) < static_cast<int>(a.units)) ++a.lanes_log2;
-  const uint32_t at_once = kThreads >> a.lanes_log2;
-  // Four rows a lane, but enough blocks for two on every SM first.
-  const uint32_t sms = static_cast<uint32_t>(ctx->sm_count);
-  a.tile = std::min(std::max(4 * at_once / a.heads, 1u), kMaxTile);
-  while (a.tile > 1 && (a.tokens + a.tile - 1) / a.tile < 2 * sms) a.tile /= 2;
-  const uint32_t tiles = (a.tokens + a.tile - 1) / a.tile;
-  const uint32_t grid = kNorm && kBack ? std::min(tiles, std::min(3 * sms, kMaxPartials)) : tiles;
-  const size_t smem = static_cast<size_t>(a.tile) * ((a.rot / 2 + V - 1) / V) * V * sizeof(float2);
-  b200::launch(ctx, rotary_kernel<T, V, kLayout, kNorm, kBack>, dim3(grid), dim3(kThreads), smem, s, 1u, a);
-  return static_cast<int>(grid);
+  while ((kUnitsOf<V> << a.lanes_log2) < static_cast<int>(a.units)) ++a.lanes_log2;
+  const uint32_t groups_log2 = 8 - a.lanes_log2, sms = static_cast<uint32_t>(ctx->sm_count);
+  static_assert(kThreads == 256, "2^8");
+  if (!kNorm) a.heads_q = a.heads;
+  const uint32_t heads_k = a.heads - a.heads_q;
+  constexpr bool kSums = kNorm && kBack;
+  // A group takes kHeadsEach heads of its token at least, one after the other, unless there are so few tokens that two blocks for
+  // every SM need them apart.
+  auto split_of = [&](uint32_t heads) {
+    uint32_t split = 0;
+    while (split < groups_log2 && ((heads >> (split + 1)) >= kHeadsEach ||
+                                   ((heads >> split) > 1 && (static_cast<u64>(a.tokens) << split) >> groups_log2 < 2 * sms)))
+      ++split;
+    return split;
+  };
+  a.split_q_log2 = split_of(a.heads_q), a.split_k_log2 = split_of(heads_k);
+  auto tiles_of = [&](uint32_t split) { return (a.tokens + (1u << (groups_log2 - split)) - 1) >> (groups_log2 - split); };
+  a.blocks_q = a.heads_q ? tiles_of(a.split_q_log2) : 0u;
+  uint32_t blocks_k = heads_k ? tiles_of(a.split_k_log2) : 0u;
+  if (kSums) {   // as many as are resident at a time, shared out by heads
+    const uint32_t room = std::min(kSumBlocks * sms, kMaxPartials);
+    const uint32_t mine = std::max(1u, static_cast<uint32_t>(static_cast<u64>(room) * a.heads_q / a.heads));
+    if (a.blocks_q) a.blocks_q = std::min(a.blocks_q, heads_k ? std::min(mine, room - 1) : room);
+    blocks_k = std::min(blocks_k, room - a.blocks_q);
+  }
+  const uint32_t most = 1u << (groups_log2 - std::min(a.heads_q ? a.split_q_log2 : groups_log2, heads_k ? a.split_k_log2 : groups_log2));
+  const size_t smem = static_cast<size_t>(most) * ((a.rot / 2 + V - 1) / V) * V * sizeof(float2);
+  b200::launch(ctx, rotary_kernel<T, V, kLayout, kNorm, kBack>, dim3(a.blocks_q + blocks_k), dim3(kThreads), smem, s, 1u, a);
+  *rows_q = a.blocks_q;
+  return static_cast<int>(a.blocks_q + blocks_k);
 }
 
 template <typename T, int kLayout, bool kNorm, bool kBack>
-int launch_rotary_v(b200_ctx *ctx, cudaStream_t s, const RotaryArgs &a) {
+int launch_rotary_v(b200_ctx *ctx, cudaStream_t s, const RotaryArgs &a, uint32_t *rows_q) {
   switch (vector_width<T>(a, kLayout, kBack, kNorm)) {
-    case 8: if constexpr (sizeof(T) == 2) return launch_rotary<T, 8, kLayout, kNorm, kBack>(ctx, s, a);
-    case 4: return launch_rotary<T, 4, kLayout, kNorm, kBack>(ctx, s, a);
-    case 2: return launch_rotary<T, 2, kLayout, kNorm, kBack>(ctx, s, a);
-    default: return launch_rotary<T, 1, kLayout, kNorm, kBack>(ctx, s, a);
+    case 8: if constexpr (sizeof(T) == 2 && !kNorm) return launch_rotary<T, 8, kLayout, kNorm, kBack>(ctx, s, a, rows_q);
+    case 4: return launch_rotary<T, 4, kLayout, kNorm, kBack>(ctx, s, a, rows_q);
+    case 2: return launch_rotary<T, 2, kLayout, kNorm, kBack>(ctx, s, a, rows_q);
+    default: return launch_rotary<T, 1, kLayout, kNorm, kBack>(ctx, s, a, rows_q);
   }
 }
 
 template <typename T, bool kNorm, bool kBack>
-int launch_rotary_l(b200_ctx *ctx, cudaStream_t s, const RotaryArgs &a, int layout) {
-  return layout == B200_ROTARY_HALVES ? launch_rotary_v<T, B200_ROTARY_HALVES, kNorm, kBack>(ctx, s, a)
-                                      : launch_rotary_v<T, B200_ROTARY_PAIRS, kNorm, kBack>(ctx, s, a);
+int launch_rotary_l(b200_ctx *ctx, cudaStream_t s, const RotaryArgs &a, int layout, uint32_t *rows_q) {
+  return layout == B200_ROTARY_HALVES ? launch_rotary_v<T, B200_ROTARY_HALVES, kNorm, kBack>(ctx, s, a, rows_q)
+                                      : launch_rotary_v<T, B200_ROTARY_PAIRS, kNorm, kBack>(ctx, s, a, rows_q);
 }
 
 // What every entry point refuses; fills in dense strides.
@@ -355,7 +509,7 @@ int check(RotaryArgs *a, int layout, bool norm) {
   if (layout != B200_ROTARY_PAIRS && layout != B200_ROTARY_HALVES) return B200_ERR_INVALID_ARG;
   if (a->head == 0 || a->rot > a->head || a->rot % 2 != 0 || (a->rot != 0 && !a->freqs)) return B200_ERR_INVALID_ARG;
   if (a->head > kMaxHead) return B200_ERR_TOO_LARGE;
-  if (static_cast<u64>(a->heads) * a->head > 0xffffffffu / kMaxTile) return B200_ERR_TOO_LARGE;
+  if (static_cast<u64>(a->heads) * a->head > 0x7fffffffu) return B200_ERR_TOO_LARGE;
   const u64 dense = static_cast<u64>(a->heads) * a->head;
   for (u64 *ld : {&a->x_ld, &a->g_ld, &a->y_ld}) {
     if (*ld == 0) *ld = dense;
@@ -415,7 +569,8 @@ int b200_rotary_fw(b200_ctx *ctx, int mode, const void *x, void *y, uint32_t hea
   if (heads == 0 || tokens == 0) return B200_OK;
   if (!x || !y || clash(x, a.x_ld, y, a.y_ld, 0)) return B200_ERR_INVALID_ARG;
   ProfScope prof(ctx, kProfElementwise, s);
-  B200_DISPATCH_MODE(mode, { (launch_rotary_l<T, false, false>(ctx, s, a, layout)); });
+  uint32_t rows_q = 0;
+  B200_DISPATCH_MODE(mode, { (launch_rotary_l<T, false, false>(ctx, s, a, layout, &rows_q)); });
   B200_OPS_EPILOGUE(ctx);
 }
 
@@ -430,7 +585,8 @@ int b200_rotary_bw(b200_ctx *ctx, int mode, const void *gy, void *gx, uint32_t h
   if (heads == 0 || tokens == 0) return B200_OK;
   if (!gy || !gx || clash(gy, a.g_ld, gx, a.y_ld, accumulate)) return B200_ERR_INVALID_ARG;
   ProfScope prof(ctx, kProfElementwise, s);
-  B200_DISPATCH_MODE(mode, { (launch_rotary_l<T, false, true>(ctx, s, a, layout)); });
+  uint32_t rows_q = 0;
+  B200_DISPATCH_MODE(mode, { (launch_rotary_l<T, false, true>(ctx, s, a, layout, &rows_q)); });
   B200_OPS_EPILOGUE(ctx);
 }
 
@@ -446,7 +602,8 @@ int b200_norm_rotary_fw(b200_ctx *ctx, int mode, const void *x, const void *gain
   if (a.heads == 0 || tokens == 0) return B200_OK;
   if (!x || !y || clash(x, a.x_ld, y, a.y_ld, 0)) return B200_ERR_INVALID_ARG;
   ProfScope prof(ctx, kProfElementwise, s);
-  B200_DISPATCH_MODE(mode, { (launch_rotary_l<T, true, false>(ctx, s, a, layout)); });
+  uint32_t rows_q = 0;
+  B200_DISPATCH_MODE(mode, { (launch_rotary_l<T, true, false>(ctx, s, a, layout, &rows_q)); });
   B200_OPS_EPILOGUE(ctx);
 }
 
@@ -467,10 +624,11 @@ int b200_norm_rotary_bw(b200_ctx *ctx, int mode, const void *x, const void *gain
   if (none && (!sums || accumulate_gain)) return B200_OK;
   a.partial = sums ? scratch : nullptr;
   ProfScope prof(ctx, kProfElementwise, s);
+  uint32_t rows_q = 0;
   B200_DISPATCH_MODE(mode, {
-    const int rows = none ? 0 : launch_rotary_l<T, true, true>(ctx, s, a, layout);
+    const int rows = none ? 0 : launch_rotary_l<T, true, true>(ctx, s, a, layout, &rows_q);
     if (sums) {
-      b200::launch(ctx, gain_sums_kernel<T>, dim3((2 * head + 31) / 32), dim3(32, 32), 0, s, 1u, scratch, rows, head,
+      b200::launch(ctx, gain_sums_kernel<T>, dim3((2 * head + 31) / 32), dim3(32, 32), 0, s, 1u, scratch, rows_q, rows, head,
                    static_cast<T *>(ggain_q), static_cast<T *>(ggain_k), accumulate_gain);
       if (!none) ++ctx->launches;
     }
