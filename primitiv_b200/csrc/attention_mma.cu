@@ -6,7 +6,7 @@
 // r / group, head r % group.
 //
 // forward:  the running maximum m and sum l of a softmax; y = y 2^(m - m') + p v, one pass over the keys.
-// backward: p is computed again from lse.  Two kernels of the same shape, one with the keys at rest (gk, gv), one with
+// backward: p is computed again from lse.  Blocks of two kinds and one shape, with the keys at rest (gk, gv) and with
 //   the queries (gq): s and dp are computed twice, which costs 7 products instead of 5 and needs neither atomics nor
 //   a sum over blocks, so the same call has the same bits.
 //
@@ -132,7 +132,9 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
 
 template <typename T, int kD> constexpr int kBwCols = sizeof(T) == 2 && kD == 64 ? 64 : 32;
 template <typename T, int kD> constexpr int kBwThreads = kD == 256 ? 256 : 128;   // 256 columns: a warp has half of them
-template <typename T, int kD> constexpr int kBwStages = sizeof(T) == 4 && kD == 256 ? 1 : 2;
+// fp32: one stage, so that more blocks share an SM: two stages took 524 us for a training step of 8 x 509 tokens, 8 heads of 64, where one takes FP32TIME.
+template <typename T, int kD> constexpr int kBwStages = sizeof(T) == 4 ? 1 : 2;
+template <typename T, int kD> constexpr int kBwBlocks = sizeof(T) == 4 && kD == 64 ? 4 : 1;
 
 // The power of two that takes the largest |ds| possible to at most 2^14.  |dp - delta| <= |gy| |v| + |delta|.
 __device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) {
@@ -143,8 +145,7 @@ __device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) 
 
 // kKeys: the keys rest, the queries of all heads of the group pass by (gk, gv).  Else the queries rest (gq).
 template <typename T, int kD, int kPass, bool kKeys>
-__global__ void __launch_bounds__(kBwThreads<T, kD>) attention_bw_kernel(AttnArgs a, uint32_t tiles, int wide) {
-  pdl_enter();
+__device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nth, uint32_t tiles, int wide) {
   constexpr int BN = kBwCols<T, kD>, NT = BN / 8, P = kPitch<T, kD>, kThreads = kBwThreads<T, kD>, kStages = kBwStages<T, kD>;
   constexpr int kCols = kD == 256 ? 128 : kD;
   constexpr bool kHalf = sizeof(T) == 2;
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(kBwThreads<T, kD>) attention_bw_kernel(AttnArg
   __shared__ float s_lse[2][BN], s_delta[2][BN], s_max[3][8];
   T *x1 = reinterpret_cast<T *>(s_raw), *x2 = x1 + kRows * P, *y1 = x2 + kRows * P, *y2 = y1 + kStages * BN * P;
   uint32_t seq, tile;
-  if (!attn_find_tile<kKeys>(a, kKeys ? blockIdx.x : tiles - 1u - blockIdx.x, kKeys ? 1u : a.group, kRows, s_at, seq, tile)) return;
+  if (!attn_find_tile<kKeys>(a, kKeys ? nth : tiles - 1u - nth, kKeys ? 1u : a.group, kRows, s_at, seq, tile)) return;
   const AttnSeq q = attn_seq(a, seq);
   const uint32_t hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
   const uint32_t wrow = (warp & 3u) * 16u, col0 = (warp >> 2) * kCols;
@@ -294,6 +295,14 @@ __global__ void __launch_bounds__(kBwThreads<T, kD>) attention_bw_kernel(AttnArg
   }
 }
 
+// Both sides in one launch: either alone leaves SMs idle behind its last blocks.
+template <typename T, int kD, int kPass>
+__global__ void __launch_bounds__(kBwThreads<T, kD>, kBwBlocks<T, kD>) attention_bw_kernel(AttnArgs a, uint32_t k_tiles, uint32_t q_tiles, int wide) {
+  pdl_enter();
+  if (blockIdx.x < k_tiles) attention_bw_side<T, kD, kPass, true>(a, blockIdx.x, k_tiles, wide);
+  else attention_bw_side<T, kD, kPass, false>(a, blockIdx.x - k_tiles, q_tiles, wide);
+}
+
 // ---- launches ----------------------------------------------------------------------------------------------
 
 template <typename T, int kD, int kPass>
@@ -306,16 +315,15 @@ int launch_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
   return B200_OK;
 }
 
-template <typename T, int kD, int kPass, bool kKeys>
-int launch_bw_side(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
+template <typename T, int kD, int kPass>
+int launch_bw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
   constexpr size_t smem = sizeof(T) * kPitch<T, kD> * (2 * kRows + 2 * kBwStages<T, kD> * kBwCols<T, kD>);
-  const uint32_t tiles = static_cast<uint32_t>(kKeys ? attn_tile_bound(a.rows_k, a.max_k, a.seqs, 1, kRows)
-                                                     : attn_tile_bound(a.rows_q, a.max_q, a.seqs, a.group, kRows));
-  if (tiles == 0) return B200_OK;
-  auto kernel = attention_bw_kernel<T, kD, kPass, kKeys>;
+  const uint32_t k_tiles = static_cast<uint32_t>(attn_tile_bound(a.rows_k, a.max_k, a.seqs, 1, kRows));
+  const uint32_t q_tiles = static_cast<uint32_t>(attn_tile_bound(a.rows_q, a.max_q, a.seqs, a.group, kRows));
+  if (k_tiles + q_tiles == 0) return B200_OK;
+  auto kernel = attention_bw_kernel<T, kD, kPass>;
   if (const int rc = allow_smem(kernel, smem)) return rc;
-  b200::launch(ctx, kernel, dim3(tiles, a.heads_k), dim3(kBwThreads<T, kD>), smem, s, 1u, a, tiles, find_wide(a, sizeof(T)));
-  ++ctx->launches;
+  b200::launch(ctx, kernel, dim3(k_tiles + q_tiles, a.heads_k), dim3(kBwThreads<T, kD>), smem, s, 1u, a, k_tiles, q_tiles, find_wide(a, sizeof(T)));
   return B200_OK;
 }
 
@@ -332,11 +340,7 @@ int attention_mma_bw(b200_ctx *ctx, int mode, const AttnArgs &a, cudaStream_t s)
   return with_type(mode, [&](auto type, auto pass) {
     using T = decltype(type);
     return with_head<T, decltype(pass)::value>(a.head, [&](auto d) {
-      constexpr int kD = decltype(d)::value, kPass = decltype(pass)::value;
-      if (const int rc = launch_bw_side<T, kD, kPass, true>(ctx, a, s)) return rc;
-      if (const int rc = launch_bw_side<T, kD, kPass, false>(ctx, a, s)) return rc;
-      --ctx->launches;   // the entry point counts the last one
-      return static_cast<int>(B200_OK);
+      return launch_bw<T, decltype(d)::value, decltype(pass)::value>(ctx, a, s);
     });
   });
 }

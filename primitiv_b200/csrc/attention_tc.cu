@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
 
 // ---- backward -----------------------------------------------------------------------------------------------
 //
-// Two kernels of one shape, as in attention_mma.cu, so that neither needs atomics: with 128 keys at rest (gk and gv; the queries of
+// Blocks of two kinds and one shape, as in attention_mma.cu, so that no sum needs atomics: with 128 keys at rest (gk and gv; the queries of
 // all heads of the group pass by) and with 128 queries at rest (gq; the keys pass by).  X1, X2 rest, tiles Y1, Y2 come
 // through a ring:
 //   keys at rest     X1 = k, X2 = v, Y1 = q, Y2 = gy:   s' = k q^T, dp' = v gy^T,  gv += p' gy,  gk += ds' q
@@ -465,16 +465,16 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
 // allow, over all that the block sees (keys at rest) or per query: without it the ds of long rows lie below the smallest half.
 
 struct alignas(64) BwParams {
-  CUtensorMap x1, x2, y1, y2;
+  CUtensorMap q, k, v, gy;
   AttnArgs a;
-  uint32_t tiles, columns;
+  uint32_t q_tiles, k_blocks;   // tiles of queries of all sequences (a bound); blocks with keys at rest, which come first
   int *status;
 };
 
 constexpr uint32_t kBwThreads = 384;
 constexpr float kPBits = 13.f;
 // Slots of the rings.  Y1 is needed first and given back last, by the product that ends a step: with two slots its copy started a step
-// late, and a step of the gq kernel took 3500 clocks instead of 1900.
+// late, and a step with queries at rest took 3500 clocks instead of 1900.
 template <int kD> constexpr uint32_t kY1 = kD == 128 ? 3u : 4u;
 template <int kD> constexpr uint32_t kY2 = kD == 128 ? 2u : 3u;
 constexpr uint32_t kStats = 2;
@@ -513,17 +513,15 @@ __device__ __forceinline__ void stat4(const float *p, f32x2 &a, f32x2 &b) {
 }
 
 template <int kD, bool kKeys>
-__global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __grid_constant__ BwParams p) {
+__device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *smem_raw) {
   constexpr uint32_t kBytes = kTile * kD * 2, kChunks = kD / 64, kSlots1 = kY1<kD>, kSlots2 = kY2<kD>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  pdl_release_next();
   BwShared &sh = *reinterpret_cast<BwShared *>(smem_raw);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint32_t smem = smem_u32(smem_raw) + kBwHead, ring1 = smem + 2 * kBytes, ring2 = ring1 + kSlots1 * kBytes;
   volatile int *abort_flag = &sh.abort;
   const AttnArgs &a = p.a;
   if (threadIdx.x == 32u) {
-    for (const CUtensorMap *m : {&p.x1, &p.x2, &p.y1, &p.y2}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(m)) : "memory");
+    for (const CUtensorMap *m : {&p.q, &p.k, &p.v, &p.gy}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(m)) : "memory");
   }
   if (threadIdx.x == 0) {
     sh.abort = 0;
@@ -540,9 +538,10 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
   pdl_wait_previous();
   tc_fence_before();
   // heaviest first: the first keys of a causal sequence are seen by the most queries, its last queries see the most keys
-  const uint32_t column = blockIdx.x % p.columns, nth = blockIdx.x / p.columns;
+  const uint32_t block = kKeys ? blockIdx.x : blockIdx.x - p.k_blocks, columns = kKeys ? a.heads_k : a.heads_q;
+  const uint32_t column = block % columns, nth = block / columns;
   uint32_t seq, tile;
-  const bool any = attn_find_tile<kKeys>(a, kKeys ? nth : p.tiles - 1u - nth, 1, kTile, sh.at, seq, tile);
+  const bool any = attn_find_tile<kKeys>(a, kKeys ? nth : p.q_tiles - 1u - nth, 1, kTile, sh.at, seq, tile);
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   // columns of tensor memory.  Keys at rest: s and then dp, p, ds, two sums; queries at rest: s, two of dp and ds, the sum
@@ -606,8 +605,8 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
         if (lane == 0) {
           mbar_arrive_expect_tx(smem_u32(&sh.x_full), 2 * kBytes);
           for (uint32_t c = 0; c < kChunks; ++c) {
-            tma_load_3d(smem + c * kChunk, &p.x1, smem_u32(&sh.x_full), c * 64, x_head, x_row);
-            tma_load_3d(smem + kBytes + c * kChunk, &p.x2, smem_u32(&sh.x_full), c * 64, x_head, x_row);
+            tma_load_3d(smem + c * kChunk, kKeys ? &p.k : &p.q, smem_u32(&sh.x_full), c * 64, x_head, x_row);
+            tma_load_3d(smem + kBytes + c * kChunk, kKeys ? &p.v : &p.gy, smem_u32(&sh.x_full), c * 64, x_head, x_row);
           }
         }
         __syncwarp();
@@ -624,10 +623,10 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
         };
         for (uint32_t i = 0; i < steps; ++i) {
           if (!wait_all(smem_u32(&sh.empty1[s1.at]), s1.phase ^ 1u, abort_flag)) break;
-          copy(&p.y1, smem_u32(&sh.full1[s1.at]), ring1 + s1.at * kBytes);
+          copy(kKeys ? &p.q : &p.k, smem_u32(&sh.full1[s1.at]), ring1 + s1.at * kBytes);
           armed1 |= 1u << s1.at, parity1 = (parity1 & ~(1u << s1.at)) | (s1.phase << s1.at);
           if (!wait_all(smem_u32(&sh.empty2[s2.at]), s2.phase ^ 1u, abort_flag)) break;
-          copy(&p.y2, smem_u32(&sh.full2[s2.at]), ring2 + s2.at * kBytes);
+          copy(kKeys ? &p.gy : &p.v, smem_u32(&sh.full2[s2.at]), ring2 + s2.at * kBytes);
           armed2 |= 1u << s2.at, parity2 = (parity2 & ~(1u << s2.at)) | (s2.phase << s2.at);
           if (++t == per) t = 0, ++g;
           s1.next(), s2.next();
@@ -907,6 +906,15 @@ __global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __
   }
 }
 
+// Both kinds in one launch: either alone leaves SMs idle behind its last blocks.
+template <int kD>
+__global__ void __launch_bounds__(kBwThreads, 1) attention_bw_tc_kernel(const __grid_constant__ BwParams p) {
+  pdl_release_next();   // (pdl_wait_previous(); comes behind the set-up, in either)
+  extern __shared__ __align__(1024) uint8_t bw_smem[];
+  if (blockIdx.x < p.k_blocks) attention_bw_side<kD, true>(p, bw_smem);
+  else attention_bw_side<kD, false>(p, bw_smem);
+}
+
 // ---- launches ------------------------------------------------------------------------------------------------
 
 // Shape({head, heads, rows}) in boxes of 64 elements of one head of 128 rows; what lies past the head or the rows reads as zero.
@@ -930,14 +938,12 @@ int launch_fw(b200_ctx *ctx, const FwParams &p, cudaStream_t s) {
   return B200_OK;
 }
 
-template <int kD, bool kKeys>
-int launch_bw(b200_ctx *ctx, const BwParams &p, cudaStream_t s) {
-  if (p.tiles == 0) return B200_OK;
-  auto kernel = attention_bw_tc_kernel<kD, kKeys>;
+template <int kD>
+int launch_bw(b200_ctx *ctx, const BwParams &p, uint32_t blocks, cudaStream_t s) {
+  auto kernel = attention_bw_tc_kernel<kD>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBwSmem<kD>));
   if (e != cudaSuccess) return static_cast<int>(e);
-  b200::launch(ctx, kernel, dim3(p.tiles * p.columns), dim3(kBwThreads), kBwSmem<kD>, s, 1u, p);
-  ++ctx->launches;
+  b200::launch(ctx, kernel, dim3(blocks), dim3(kBwThreads), kBwSmem<kD>, s, 1u, p);
   return B200_OK;
 }
 
@@ -972,24 +978,20 @@ bool attention_tc_bw_eligible(const b200_ctx *ctx, int mode, const AttnArgs &a) 
 }
 
 int attention_tc_bw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
-  CUtensorMap q, k, v, gy;
-  int rc = encode(ctx, &q, a.q, a.head, a.heads_q, a.rows_q, a.q_ld);
-  if (rc == B200_OK) rc = encode(ctx, &k, a.k, a.head, a.heads_k, a.rows_k, a.k_ld);
-  if (rc == B200_OK) rc = encode(ctx, &v, a.v, a.head, a.heads_k, a.rows_k, a.v_ld);
-  if (rc == B200_OK) rc = encode(ctx, &gy, a.gy, a.head, a.heads_q, a.rows_q, a.y_ld);
-  if (rc != B200_OK) return rc;
-  const unsigned long long k_tiles = attn_tile_bound(a.rows_k, a.max_k, a.seqs, 1, kTile), q_tiles = attn_tile_bound(a.rows_q, a.max_q, a.seqs, 1, kTile);
-  if (k_tiles * a.heads_k > 0x7fffffffull || q_tiles * a.heads_q > 0x7fffffffull) return B200_ERR_TOO_LARGE;
   BwParams p;
   std::memset(&p, 0, sizeof(p));
   p.a = a, p.status = ctx->d_status;
-  p.x1 = k, p.x2 = v, p.y1 = q, p.y2 = gy, p.tiles = static_cast<uint32_t>(k_tiles), p.columns = a.heads_k;
-  rc = a.head <= 64 ? launch_bw<64, true>(ctx, p, s) : launch_bw<128, true>(ctx, p, s);
+  int rc = encode(ctx, &p.q, a.q, a.head, a.heads_q, a.rows_q, a.q_ld);
+  if (rc == B200_OK) rc = encode(ctx, &p.k, a.k, a.head, a.heads_k, a.rows_k, a.k_ld);
+  if (rc == B200_OK) rc = encode(ctx, &p.v, a.v, a.head, a.heads_k, a.rows_k, a.v_ld);
+  if (rc == B200_OK) rc = encode(ctx, &p.gy, a.gy, a.head, a.heads_q, a.rows_q, a.y_ld);
   if (rc != B200_OK) return rc;
-  p.x1 = q, p.x2 = gy, p.y1 = k, p.y2 = v, p.tiles = static_cast<uint32_t>(q_tiles), p.columns = a.heads_q;
-  rc = a.head <= 64 ? launch_bw<64, false>(ctx, p, s) : launch_bw<128, false>(ctx, p, s);
-  --ctx->launches;   // the entry point counts the last one
-  return rc;
+  const unsigned long long k_tiles = attn_tile_bound(a.rows_k, a.max_k, a.seqs, 1, kTile), q_tiles = attn_tile_bound(a.rows_q, a.max_q, a.seqs, 1, kTile);
+  const unsigned long long blocks = k_tiles * a.heads_k + q_tiles * a.heads_q;
+  if (blocks > 0x7fffffffull) return B200_ERR_TOO_LARGE;
+  if (blocks == 0) return B200_OK;
+  p.q_tiles = static_cast<uint32_t>(q_tiles), p.k_blocks = static_cast<uint32_t>(k_tiles * a.heads_k);
+  return a.head <= 64 ? launch_bw<64>(ctx, p, static_cast<uint32_t>(blocks), s) : launch_bw<128>(ctx, p, static_cast<uint32_t>(blocks), s);
 }
 
 }  // namespace b200
