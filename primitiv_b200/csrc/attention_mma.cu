@@ -10,6 +10,9 @@
 //   the queries (gq): s and dp are computed twice, which costs 7 products instead of 5 and needs neither atomics nor
 //   a sum over blocks, so the same call has the same bits.
 //
+// With few tiles a cluster of blocks shares each, every one with a part of what passes by; their sums are joined through distributed
+// shared memory, in rank order.
+//
 // fp32 storage: a product is three TF32 passes on x = hi + lo split in registers (one in B200_MODE_TF32).  The tensor core
 // truncates as it adds into its accumulator, so no sum runs longer than one tile there: each tile's product starts from zero and
 // is added in fp32 instructions.  Halves: p and ds are rounded to half for the second product, ds after a scale by a power of
@@ -17,6 +20,7 @@
 // smallest half.
 #include <algorithm>
 #include "attention_mma.cuh"
+#include "tcgen05.cuh"
 
 namespace b200 {
 namespace {
@@ -29,15 +33,17 @@ constexpr float kPScale = 8192.f;    // backward, halves: p in [0, 1] times this
 template <typename T, int kD> constexpr int kFwCols = sizeof(T) == 2 ? 64 : 32;
 
 template <typename T, int kD, int kPass>
-__global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t tiles, int wide) {
+__global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t tiles, uint32_t splits, int wide) {
   pdl_enter();
   constexpr int BN = kFwCols<T, kD>, NT = BN / 8, P = kPitch<T, kD>;
   extern __shared__ __align__(16) unsigned char s_raw[];
   __shared__ uint32_t s_at[2];
   T *sq = reinterpret_cast<T *>(s_raw), *sk = sq + kRows * P, *sv = sk + 2 * BN * P;
+  __shared__ float s_m[kRows], s_l[kRows];
+  const uint32_t rank = splits > 1 ? blockIdx.x % splits : 0u;
   // the last tiles of a causal sequence have the most keys: they go first
   uint32_t seq, tile;
-  if (!attn_find_tile<false>(a, tiles - 1u - blockIdx.x, a.group, kRows, s_at, seq, tile)) return;
+  if (!attn_find_tile<false>(a, tiles - 1u - blockIdx.x / splits, a.group, kRows, s_at, seq, tile)) return;   // the whole cluster
   const AttnSeq q = attn_seq(a, seq);
   const uint32_t hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
   const uint32_t rows = q.lq * a.group, row0 = tile * kRows;
@@ -50,12 +56,13 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
     const long long seen = static_cast<long long>((min(row0 + kRows, rows) - 1u) / a.group) + shift + 1;
     keys = seen <= 0 ? 0u : min(keys, static_cast<uint32_t>(seen));
   }
-  const uint32_t steps = (keys + BN - 1) / BN;
+  const uint32_t all_steps = (keys + BN - 1) / BN, share = (all_steps + splits - 1) / splits;   // steps of one block of the cluster
+  const uint32_t step0 = min(rank * share, all_steps), steps = min(step0 + share, all_steps) - step0, first_key = step0 * BN;
 
   load_rows<T, kD, kRows, 128>(sq, qb, a.q_ld, a.group, row0, rows, a.head, wide & kWideQ);
   if (steps) {
-    load_rows<T, kD, BN, 128>(sk, kb, a.k_ld, 1, 0, keys, a.head, wide & kWideK);
-    load_rows<T, kD, BN, 128>(sv, vb, a.v_ld, 1, 0, keys, a.head, wide & kWideV);
+    load_rows<T, kD, BN, 128>(sk, kb, a.k_ld, 1, first_key, keys, a.head, wide & kWideK);
+    load_rows<T, kD, BN, 128>(sv, vb, a.v_ld, 1, first_key, keys, a.head, wide & kWideV);
   }
   copies_commit();
 
@@ -79,14 +86,14 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
     copies_wait<0>();
     __syncthreads();
     if (step + 1 < steps) {
-      const uint32_t next = (step + 1) * BN;
+      const uint32_t next = first_key + (step + 1) * BN;
       load_rows<T, kD, BN, 128>(sk + (at ^ 1u) * BN * P, kb, a.k_ld, 1, next, keys, a.head, wide & kWideK);
       load_rows<T, kD, BN, 128>(sv + (at ^ 1u) * BN * P, vb, a.v_ld, 1, next, keys, a.head, wide & kWideV);
       copies_commit();
     }
     float s[NT][4];
     product_abt<kD, NT, kPass>(s, sq + warp * 16 * P, sk + at * BN * P);
-    const uint32_t key0 = step * BN;
+    const uint32_t key0 = first_key + step * BN;
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -116,6 +123,43 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
     }
     product_py<kD, kD, NT, kPass>(acc, s, sv + at * BN * P, 0, keep[0], keep[1]);
   }
+  if (splits > 1) {
+    // the blocks' parts: each lays down its own, and joins the rows that fall to it, in rank order
+    float *part = reinterpret_cast<float *>(sk);
+    copies_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t at = warp * 16 + g + r * 8;
+      l[r] = quad_sum(l[r]);
+      if (t == 0) s_m[at] = m[r], s_l[at] = l[r];
+#pragma unroll
+      for (int n = 0; n < kD / 8; ++n) *reinterpret_cast<float2 *>(part + at * kD + n * 8 + 2 * t) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+    }
+    cluster_sync_all();
+    const uint32_t mine = kRows / splits, at0 = rank * mine;
+    for (uint32_t i = threadIdx.x; i < mine * (kD / 4); i += 128) {
+      const uint32_t at = at0 + i / (kD / 4), c = i % (kD / 4) * 4, rw = row0 + at;
+      if (rw >= rows || c >= a.head) continue;
+      float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, ld_cluster(map_to_cta(smem_at(s_m + at), s)));
+      for (uint32_t s = 0; s < splits; ++s) {
+        const float ms = ld_cluster(map_to_cta(smem_at(s_m + at), s)), w = ms == -INFINITY ? 0.f : exp2_of<T>(ms - top);
+        const float4 o = ld_cluster4(map_to_cta(smem_at(part + at * kD + c), s));
+        sum += w * ld_cluster(map_to_cta(smem_at(s_l + at), s));
+        v[0] += w * o.x, v[1] += w * o.y, v[2] += w * o.z, v[3] += w * o.w;
+      }
+      const bool any = top != -INFINITY;
+      const uint32_t tok = rw / a.group, h = hk * a.group + rw - tok * a.group;
+      T *out = static_cast<T *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(h) * a.head + c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < a.head) out[e] = round_to<T>(any ? v[e] / sum : v[e]);   // (a sum of zeros, or a NaN)
+      if (a.lse && c == 0) a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = any ? top * kLn2 + logf(sum) : sum - INFINITY;
+    }
+    cluster_sync_all();   // nobody leaves while another reads its part
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] = quad_sum(l[r]);
@@ -132,9 +176,10 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
 
 template <typename T, int kD> constexpr int kBwCols = sizeof(T) == 2 && kD == 64 ? 64 : 32;
 template <typename T, int kD> constexpr int kBwThreads = kD == 256 ? 256 : 128;   // 256 columns: a warp has half of them
-// fp32: one stage, so that more blocks share an SM: two stages took 524 us for a training step of 8 x 509 tokens, 8 heads of 64, where one takes FP32TIME.
+// fp32: one stage, so that more blocks share an SM.  A training step of 8 x 509 tokens, 8 heads of 64: 435 us; with two stages 470, with four blocks to an
+// SM (128 registers, some in memory) 452.
 template <typename T, int kD> constexpr int kBwStages = sizeof(T) == 4 ? 1 : 2;
-template <typename T, int kD> constexpr int kBwBlocks = sizeof(T) == 4 && kD == 64 ? 4 : 1;
+template <typename T, int kD> constexpr int kBwBlocks = sizeof(T) == 4 && kD == 64 ? 3 : 1;
 
 // The power of two that takes the largest |ds| possible to at most 2^14.  |dp - delta| <= |gy| |v| + |delta|.
 __device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) {
@@ -145,16 +190,18 @@ __device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) 
 
 // kKeys: the keys rest, the queries of all heads of the group pass by (gk, gv).  Else the queries rest (gq).
 template <typename T, int kD, int kPass, bool kKeys>
-__device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nth, uint32_t tiles, int wide) {
+__device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nth, uint32_t tiles, uint32_t splits, int wide) {
   constexpr int BN = kBwCols<T, kD>, NT = BN / 8, P = kPitch<T, kD>, kThreads = kBwThreads<T, kD>, kStages = kBwStages<T, kD>;
   constexpr int kCols = kD == 256 ? 128 : kD;
   constexpr bool kHalf = sizeof(T) == 2;
   extern __shared__ __align__(16) unsigned char s_raw[];
   __shared__ uint32_t s_at[2];
   __shared__ float s_lse[2][BN], s_delta[2][BN], s_max[3][8];
+  __shared__ int s_last[2][BN];   // the last key that a query sees
   T *x1 = reinterpret_cast<T *>(s_raw), *x2 = x1 + kRows * P, *y1 = x2 + kRows * P, *y2 = y1 + kStages * BN * P;
   uint32_t seq, tile;
-  if (!attn_find_tile<kKeys>(a, kKeys ? nth : tiles - 1u - nth, kKeys ? 1u : a.group, kRows, s_at, seq, tile)) return;
+  if (!attn_find_tile<kKeys>(a, kKeys ? nth : tiles - 1u - nth, kKeys ? 1u : a.group, kRows, s_at, seq, tile)) return;   // the whole cluster
+  const uint32_t rank = splits > 1 ? blockIdx.x % splits : 0u;
   const AttnSeq q = attn_seq(a, seq);
   const uint32_t hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
   const uint32_t wrow = (warp & 3u) * 16u, col0 = (warp >> 2) * kCols;
@@ -174,11 +221,16 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
       to = seen <= 0 ? 0u : min(to, static_cast<uint32_t>(seen));
     }
   }
-  const uint32_t steps = to > from ? (to - from + BN - 1) / BN : 0u;
+  const uint32_t all_steps = to > from ? (to - from + BN - 1) / BN : 0u, share = (all_steps + splits - 1) / splits;   // steps of one block of the cluster
+  const uint32_t step0 = min(rank * share, all_steps), steps = min(step0 + share, all_steps) - step0;
   const unsigned long long stat = static_cast<unsigned long long>(hk) * a.group * a.rows_q + q.q0;   // of query 0, first head
 
+  auto last_key = [&](uint32_t tok) {
+    const long long see = a.causal ? min(static_cast<long long>(tok) + shift, static_cast<long long>(q.lk) - 1) : static_cast<long long>(q.lk) - 1;
+    return static_cast<int>(max(see, -1ll));
+  };
   auto load_step = [&](uint32_t step, uint32_t at) {
-    const uint32_t r0 = from + step * BN;
+    const uint32_t r0 = from + (step0 + step) * BN;
     if constexpr (kKeys) {
       load_rows<T, kD, BN, kThreads>(y1 + at * BN * P, qb, a.q_ld, a.group, r0, to, a.head, wide & kWideQ);
       load_rows<T, kD, BN, kThreads>(y2 + at * BN * P, gyb, a.y_ld, a.group, r0, to, a.head, wide & kWideGy);
@@ -186,6 +238,7 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
         const uint32_t r = r0 + threadIdx.x, tok = r / a.group;
         const unsigned long long i = stat + static_cast<unsigned long long>(r - tok * a.group) * a.rows_q + tok;
         s_lse[at][threadIdx.x] = r < to ? a.lse[i] * kLog2e : 0.f;
+        s_last[at][threadIdx.x] = r < to ? last_key(tok) : -1;
         s_delta[at][threadIdx.x] = r < to ? a.delta[i] : 0.f;
       }
     } else {
@@ -231,16 +284,17 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
   }
 
   uint32_t row[2];
+  int row_last[2];   // queries at rest: the last key that the row sees; keys at rest: the row's key
   float row_lse[2] = {0.f, 0.f}, row_delta[2] = {0.f, 0.f};
-  unsigned long long row_at[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     row[r] = row0 + wrow + g + r * 8;
     const uint32_t tok = row[r] / a.group;
-    row_at[r] = stat + static_cast<unsigned long long>(row[r] - tok * a.group) * a.rows_q + tok;
+    row_last[r] = kKeys ? static_cast<int>(row[r]) : (row[r] < rows ? last_key(tok) : -1);
     if (!kKeys && row[r] < rows) {
-      row_lse[r] = a.lse[row_at[r]] * kLog2e;
-      row_delta[r] = a.delta[row_at[r]];
+      const unsigned long long at = stat + static_cast<unsigned long long>(row[r] - tok * a.group) * a.rows_q + tok;
+      row_lse[r] = a.lse[at] * kLog2e;
+      row_delta[r] = a.delta[at];
     }
   }
   float acc1[kKeys ? kCols / 8 : 1][4], acc2[kCols / 8][4];
@@ -268,19 +322,62 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t c = n * 8 + 2 * t + (i & 1), col = from + step * BN + c, r = row[i >> 1];
-        const uint32_t key = kKeys ? r : col, qr = kKeys ? col : r;
-        const bool seen = key < q.lk && qr < qrows && (!a.causal || static_cast<long long>(key) <= static_cast<long long>(qr / a.group) + shift);
-        const float lse = kKeys ? s_lse[at][c] : row_lse[i >> 1], delta = kKeys ? s_delta[at][c] : row_delta[i >> 1];
-        const float e = seen ? exp2_of<T>(p[n][i] * to2 - lse) : 0.f;
-        ds[n][i] = seen ? e * (ds[n][i] - delta) * ds_scale : 0.f;
-        p[n][i] = kHalf ? e * kPScale : e;
+      for (int e = 0; e < 2; ++e) {
+        const int c = n * 8 + 2 * t + e, key = static_cast<int>(from + (step0 + step) * BN) + c;
+        const int col_last = kKeys ? s_last[at][c] : 0;
+        const float col_lse = kKeys ? s_lse[at][c] : 0.f, col_delta = kKeys ? s_delta[at][c] : 0.f;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int i = 2 * r + e;
+          const bool seen = kKeys ? row_last[r] <= col_last : key <= row_last[r];
+          const float x = seen ? exp2_of<T>(p[n][i] * to2 - (kKeys ? col_lse : row_lse[r])) : 0.f;
+          ds[n][i] = seen ? x * (ds[n][i] - (kKeys ? col_delta : row_delta[r])) * ds_scale : 0.f;
+          p[n][i] = kHalf ? x * kPScale : x;
+        }
       }
     if constexpr (kKeys) product_py<kD, kCols, NT, kPass>(acc1, p, y2 + at * BN * P, col0, 1.f, 1.f);
     product_py<kD, kCols, NT, kPass>(acc2, ds, y1 + at * BN * P, col0, 1.f, 1.f);
   }
   const float undo = a.scale / ds_scale;
+  if (splits > 1) {
+    // the blocks' sums: each lays down its own, and adds the rows that fall to it, in rank order
+    float *part = reinterpret_cast<float *>(s_raw);
+    copies_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int n = 0; n < kCols / 8; ++n) {
+        float *at = part + (wrow + g + r * 8) * kD + col0 + n * 8 + 2 * t;
+        *reinterpret_cast<float2 *>(at) = make_float2(acc2[n][2 * r], acc2[n][2 * r + 1]);
+        if constexpr (kKeys) *reinterpret_cast<float2 *>(at + kRows * kD) = make_float2(acc1[n][2 * r], acc1[n][2 * r + 1]);
+      }
+    cluster_sync_all();
+    const uint32_t mine = kRows / splits, at0 = rank * mine;
+    for (uint32_t i = threadIdx.x; i < (kKeys ? 2u : 1u) * mine * (kD / 4); i += kThreads) {
+      const uint32_t which = i / (mine * (kD / 4)), in = i - which * mine * (kD / 4);   // gk or gq, then gv
+      const uint32_t at = at0 + in / (kD / 4), c = in % (kD / 4) * 4, rw = row0 + at;
+      if (rw >= rows || c >= a.head) continue;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (uint32_t s = 0; s < splits; ++s) {
+        const float4 o = ld_cluster4(map_to_cta(smem_at(part + (which * kRows + at) * kD + c), s));
+        v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
+      }
+      const float factor = which ? (kHalf ? 1.f / kPScale : 1.f) : undo;
+      T *out;
+      if constexpr (kKeys) {
+        out = which ? static_cast<T *>(a.gv) + (q.k0 + rw) * a.v_ld + hk_at : static_cast<T *>(a.gk) + (q.k0 + rw) * a.k_ld + hk_at;
+      } else {
+        const uint32_t tok = rw / a.group;
+        out = static_cast<T *>(a.gq) + (q.q0 + tok) * a.q_ld + hq_at + static_cast<unsigned long long>(rw - tok * a.group) * a.head;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < a.head) out[c + e] = round_to<T>(v[e] * factor + (a.accumulate ? static_cast<float>(out[c + e]) : 0.f));
+    }
+    cluster_sync_all();   // nobody leaves while another reads its part
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     if (row[r] >= rows) continue;
@@ -297,13 +394,21 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
 
 // Both sides in one launch: either alone leaves SMs idle behind its last blocks.
 template <typename T, int kD, int kPass>
-__global__ void __launch_bounds__(kBwThreads<T, kD>, kBwBlocks<T, kD>) attention_bw_kernel(AttnArgs a, uint32_t k_tiles, uint32_t q_tiles, int wide) {
+__global__ void __launch_bounds__(kBwThreads<T, kD>, kBwBlocks<T, kD>) attention_bw_kernel(AttnArgs a, uint32_t k_tiles, uint32_t q_tiles, uint32_t splits, int wide) {
   pdl_enter();
-  if (blockIdx.x < k_tiles) attention_bw_side<T, kD, kPass, true>(a, blockIdx.x, k_tiles, wide);
-  else attention_bw_side<T, kD, kPass, false>(a, blockIdx.x - k_tiles, q_tiles, wide);
+  const uint32_t item = blockIdx.x / splits;
+  if (item < k_tiles) attention_bw_side<T, kD, kPass, true>(a, item, k_tiles, splits, wide);
+  else attention_bw_side<T, kD, kPass, false>(a, item - k_tiles, q_tiles, splits, wide);
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------
+
+// Blocks of a cluster that share a tile: as many as bring four on every SM, while each has two steps of the longest.
+uint32_t split_of(const b200_ctx *ctx, unsigned long long blocks, unsigned long long steps) {
+  uint32_t splits = 1;
+  while (splits < 8 && blocks * splits < 4ull * ctx->sm_count && steps / (2 * splits) >= 2) splits *= 2;
+  return splits;
+}
 
 template <typename T, int kD, int kPass>
 int launch_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
@@ -311,7 +416,9 @@ int launch_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
   const uint32_t tiles = static_cast<uint32_t>(attn_tile_bound(a.rows_q, a.max_q, a.seqs, a.group, kRows));
   auto kernel = attention_fw_kernel<T, kD, kPass>;
   if (const int rc = allow_smem(kernel, smem)) return rc;
-  b200::launch(ctx, kernel, dim3(tiles, a.heads_k), dim3(128), smem, s, 1u, a, tiles, find_wide(a, sizeof(T)));
+  const uint32_t splits = split_of(ctx, static_cast<unsigned long long>(tiles) * a.heads_k, a.max_k / kFwCols<T, kD>);
+  if (static_cast<unsigned long long>(tiles) * splits > 0x7fffffffull) return B200_ERR_TOO_LARGE;
+  b200::launch(ctx, kernel, dim3(tiles * splits, a.heads_k), dim3(128), smem, s, splits, a, tiles, splits, find_wide(a, sizeof(T)));
   return B200_OK;
 }
 
@@ -323,7 +430,10 @@ int launch_bw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
   if (k_tiles + q_tiles == 0) return B200_OK;
   auto kernel = attention_bw_kernel<T, kD, kPass>;
   if (const int rc = allow_smem(kernel, smem)) return rc;
-  b200::launch(ctx, kernel, dim3(k_tiles + q_tiles, a.heads_k), dim3(kBwThreads<T, kD>), smem, s, 1u, a, k_tiles, q_tiles, find_wide(a, sizeof(T)));
+  const uint32_t splits = split_of(ctx, static_cast<unsigned long long>(k_tiles + q_tiles) * a.heads_k,
+                                   std::max<unsigned long long>(a.max_k, static_cast<unsigned long long>(a.max_q) * a.group) / kBwCols<T, kD>);
+  b200::launch(ctx, kernel, dim3((k_tiles + q_tiles) * splits, a.heads_k), dim3(kBwThreads<T, kD>), smem, s, splits, a, k_tiles, q_tiles, splits,
+               find_wide(a, sizeof(T)));
   return B200_OK;
 }
 

@@ -90,17 +90,21 @@ __device__ __forceinline__ void product_abt(float (&c)[NT][4], const float *x, c
     split<kPass>(xa[8 * P + kk * 8], ah[1], al[1]);
     split<kPass>(xa[kk * 8 + 4], ah[2], al[2]);
     split<kPass>(xa[8 * P + kk * 8 + 4], ah[3], al[3]);
+    // the passes of one sum are NT instructions apart: behind one another they wait 30 clocks each
+    uint32_t bh[NT][2], bl[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      uint32_t bh[2], bl[2];
-      split<kPass>(ya[n * 8 * P + kk * 8], bh[0], bl[0]);
-      split<kPass>(ya[n * 8 * P + kk * 8 + 4], bh[1], bl[1]);
-      if constexpr (kPass == 3) {
-        mma_tf32(c[n], al, bh[0], bh[1]);
-        mma_tf32(c[n], ah, bl[0], bl[1]);
-      }
-      mma_tf32(c[n], ah, bh[0], bh[1]);
+      split<kPass>(ya[n * 8 * P + kk * 8], bh[n][0], bl[n][0]);
+      split<kPass>(ya[n * 8 * P + kk * 8 + 4], bh[n][1], bl[n][1]);
     }
+    if constexpr (kPass == 3) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_tf32(c[n], al, bh[n][0], bh[n][1]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_tf32(c[n], ah, bl[n][0], bl[n][1]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma_tf32(c[n], ah, bh[n][0], bh[n][1]);
   }
 }
 
@@ -150,22 +154,35 @@ __device__ __forceinline__ void product_py(float (&acc)[kCols / 8][4], const flo
     split<kPass>(p[j][1], ah[j][2], al[j][2]);
     split<kPass>(p[j][3], ah[j][3], al[j][3]);
   }
+  // four sums side by side, for the same reason as above
 #pragma unroll
-  for (int n = 0; n < kCols / 8; ++n) {
-    float c[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int n0 = 0; n0 < kCols / 8; n0 += 4) {
+    float c[4][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      uint32_t bh[2], bl[2];
-      split<kPass>(ya[j * 8 * P + n * 8], bh[0], bl[0]);
-      split<kPass>(ya[j * 8 * P + P + n * 8], bh[1], bl[1]);
-      if constexpr (kPass == 3) {
-        mma_tf32(c, al[j], bh[0], bh[1]);
-        mma_tf32(c, ah[j], bl[0], bl[1]);
+      uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        split<kPass>(ya[j * 8 * P + (n0 + n) * 8], bh[n][0], bl[n][0]);
+        split<kPass>(ya[j * 8 * P + P + (n0 + n) * 8], bh[n][1], bl[n][1]);
       }
-      mma_tf32(c, ah[j], bh[0], bh[1]);
+      if constexpr (kPass == 3) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) mma_tf32(c[n], al[j], bh[n][0], bh[n][1]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) mma_tf32(c[n], ah[j], bl[n][0], bl[n][1]);
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) mma_tf32(c[n], ah[j], bh[n][0], bh[n][1]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = acc[n][i] * (i < 2 ? keep0 : keep1) + c[i];
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n0 + n][i] = acc[n0 + n][i] * (i < 2 ? keep0 : keep1) + c[n][i];
   }
 }
 
@@ -239,6 +256,18 @@ __device__ __forceinline__ float quad_sum(float v) {
 template <typename T> __device__ __forceinline__ float exp2_of(float x) {
   if constexpr (sizeof(T) == 2) return attn_exp2(x);
   else return exp2f(x);
+}
+
+// Shared memory of another block of the cluster.
+__device__ __forceinline__ float ld_cluster(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
 }
 
 enum { kWideQ = 1, kWideK = 2, kWideV = 4, kWideGy = 8 };

@@ -26,17 +26,6 @@ template <typename T, int kD> constexpr uint32_t kQueryBytes = (sizeof(T) == 2 ?
 template <typename T, int kD>
 constexpr uint32_t kSmem = std::max<uint32_t>(kWarps * kWarpBytes<T, kD>, kWarps * 16 * kD * 4) + kQueryBytes<T, kD>;
 
-__device__ __forceinline__ float ld_cluster(uint32_t at) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-  return v;
-}
-
 // s[16 rows][8 NT] = q k^T.  Halves: q in registers.
 template <int kD, int NT>
 __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&qf)[kD / 16][4], const __half *k) {
