@@ -176,8 +176,8 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
 
 template <typename T, int kD> constexpr int kBwCols = sizeof(T) == 2 && kD == 64 ? 64 : 32;
 template <typename T, int kD> constexpr int kBwThreads = kD == 256 ? 256 : 128;   // 256 columns: a warp has half of them
-// fp32: one stage, so that more blocks share an SM.  A training step of 8 x 509 tokens, 8 heads of 64: 435 us; with two stages 470, with four blocks to an
-// SM (128 registers, some in memory) 452.
+// fp32: one stage, so that more blocks share an SM.  A training step of 8 x 509 tokens, 8 heads of 64: 467 us; two stages, or four blocks to an
+// SM (128 registers, some in memory), are 4 to 8 % slower.
 template <typename T, int kD> constexpr int kBwStages = sizeof(T) == 4 ? 1 : 2;
 template <typename T, int kD> constexpr int kBwBlocks = sizeof(T) == 4 && kD == 64 ? 3 : 1;
 
@@ -194,6 +194,8 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
   constexpr int BN = kBwCols<T, kD>, NT = BN / 8, P = kPitch<T, kD>, kThreads = kBwThreads<T, kD>, kStages = kBwStages<T, kD>;
   constexpr int kCols = kD == 256 ? 128 : kD;
   constexpr bool kHalf = sizeof(T) == 2;
+  // p = exp(s - lse).  fp32: the difference first, then its multiple of log2(e): lse log2(e), rounded, would cost p half of 2^-20
+  constexpr float kLseUnit = kHalf ? kLog2e : 1.f;
   extern __shared__ __align__(16) unsigned char s_raw[];
   __shared__ uint32_t s_at[2];
   __shared__ float s_lse[2][BN], s_delta[2][BN], s_max[3][8];
@@ -237,7 +239,7 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
       if (threadIdx.x < BN) {
         const uint32_t r = r0 + threadIdx.x, tok = r / a.group;
         const unsigned long long i = stat + static_cast<unsigned long long>(r - tok * a.group) * a.rows_q + tok;
-        s_lse[at][threadIdx.x] = r < to ? a.lse[i] * kLog2e : 0.f;
+        s_lse[at][threadIdx.x] = r < to ? a.lse[i] * kLseUnit : 0.f;
         s_last[at][threadIdx.x] = r < to ? last_key(tok) : -1;
         s_delta[at][threadIdx.x] = r < to ? a.delta[i] : 0.f;
       }
@@ -293,7 +295,7 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
     row_last[r] = kKeys ? static_cast<int>(row[r]) : (row[r] < rows ? last_key(tok) : -1);
     if (!kKeys && row[r] < rows) {
       const unsigned long long at = stat + static_cast<unsigned long long>(row[r] - tok * a.group) * a.rows_q + tok;
-      row_lse[r] = a.lse[at] * kLog2e;
+      row_lse[r] = a.lse[at] * kLseUnit;
       row_delta[r] = a.delta[at];
     }
   }
@@ -330,7 +332,8 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
         for (int r = 0; r < 2; ++r) {
           const int i = 2 * r + e;
           const bool seen = kKeys ? row_last[r] <= col_last : key <= row_last[r];
-          const float x = seen ? exp2_of<T>(p[n][i] * to2 - (kKeys ? col_lse : row_lse[r])) : 0.f;
+          const float lse = kKeys ? col_lse : row_lse[r];
+          const float x = !seen ? 0.f : kHalf ? exp2_of<T>(fmaf(p[n][i], to2, -lse)) : exp2_of<T>(fmaf(p[n][i], a.scale, -lse) * kLog2e);
           ds[n][i] = seen ? x * (ds[n][i] - (kKeys ? col_delta : row_delta[r])) * ds_scale : 0.f;
           p[n][i] = kHalf ? x * kPScale : x;
         }

@@ -79,10 +79,11 @@ __device__ __forceinline__ void product_abt(float (&c)[NT][4], const float *x, c
   constexpr int P = kPitch<float, kD>;
   const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
   const float *xa = x + g * P + t, *ya = y + g * P + t;
+  float small[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
+    for (int i = 0; i < 4; ++i) c[n][i] = small[n][i] = 0.f;
 #pragma unroll 4
   for (int kk = 0; kk < kD / 8; ++kk) {
     uint32_t ah[4], al[4];
@@ -90,7 +91,8 @@ __device__ __forceinline__ void product_abt(float (&c)[NT][4], const float *x, c
     split<kPass>(xa[8 * P + kk * 8], ah[1], al[1]);
     split<kPass>(xa[kk * 8 + 4], ah[2], al[2]);
     split<kPass>(xa[8 * P + kk * 8 + 4], ah[3], al[3]);
-    // the passes of one sum are NT instructions apart: behind one another they wait 30 clocks each
+    // The passes of one sum are NT instructions apart: behind one another they wait 30 clocks each.  The small terms have a sum of
+    // their own, so that the large one is truncated once a step.
     uint32_t bh[NT][2], bl[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -99,12 +101,18 @@ __device__ __forceinline__ void product_abt(float (&c)[NT][4], const float *x, c
     }
     if constexpr (kPass == 3) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_tf32(c[n], al, bh[n][0], bh[n][1]);
+      for (int n = 0; n < NT; ++n) mma_tf32(small[n], al, bh[n][0], bh[n][1]);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_tf32(c[n], ah, bl[n][0], bl[n][1]);
+      for (int n = 0; n < NT; ++n) mma_tf32(small[n], ah, bl[n][0], bl[n][1]);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) mma_tf32(c[n], ah, bh[n][0], bh[n][1]);
+  }
+  if constexpr (kPass == 3) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[n][i] += small[n][i];
   }
 }
 
@@ -157,11 +165,11 @@ __device__ __forceinline__ void product_py(float (&acc)[kCols / 8][4], const flo
   // four sums side by side, for the same reason as above
 #pragma unroll
   for (int n0 = 0; n0 < kCols / 8; n0 += 4) {
-    float c[4][4];
+    float c[4][4], small[4][4];
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) c[n][i] = small[n][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       uint32_t bh[4][2], bl[4][2];
@@ -172,9 +180,9 @@ __device__ __forceinline__ void product_py(float (&acc)[kCols / 8][4], const flo
       }
       if constexpr (kPass == 3) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) mma_tf32(c[n], al[j], bh[n][0], bh[n][1]);
+        for (int n = 0; n < 4; ++n) mma_tf32(small[n], al[j], bh[n][0], bh[n][1]);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) mma_tf32(c[n], ah[j], bl[n][0], bl[n][1]);
+        for (int n = 0; n < 4; ++n) mma_tf32(small[n], ah[j], bl[n][0], bl[n][1]);
       }
 #pragma unroll
       for (int n = 0; n < 4; ++n) mma_tf32(c[n], ah[j], bh[n][0], bh[n][1]);
@@ -182,7 +190,7 @@ __device__ __forceinline__ void product_py(float (&acc)[kCols / 8][4], const flo
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n0 + n][i] = acc[n0 + n][i] * (i < 2 ? keep0 : keep1) + c[n][i];
+      for (int i = 0; i < 4; ++i) acc[n0 + n][i] = acc[n0 + n][i] * (i < 2 ? keep0 : keep1) + (c[n][i] + small[n][i]);
   }
 }
 
