@@ -112,7 +112,7 @@ typedef struct b200_attention {
   float scale;
 } b200_attention;
 
-/* lse: Shape({rows_q, heads_q}) of float, or NULL where no backward pass follows. */
+/* lse: Shape({rows_q, heads_q}) of float, or NULL where no backward pass follows.  y may not overlap q, k or v. */
 B200_API int b200_attention_fw(b200_ctx *ctx, int mode, const b200_attention *plan_host, const void *q, const void *k,
                                const void *v, void *y, float *lse, void *stream);
 /* gq, gk and gv from gy and from what the forward pass read and wrote.  No two of the arrays may

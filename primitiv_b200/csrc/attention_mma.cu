@@ -414,9 +414,11 @@ uint32_t split_of(const b200_ctx *ctx, unsigned long long blocks, unsigned long 
 }
 
 template <typename T, int kD, int kPass>
-int launch_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
+int launch_fw(b200_ctx *ctx, AttnArgs a, cudaStream_t s) {
   constexpr size_t smem = sizeof(T) * kPitch<T, kD> * (kRows + 4 * kFwCols<T, kD>);
-  const uint32_t tiles = static_cast<uint32_t>(attn_tile_bound(a.rows_q, a.max_q, a.seqs, a.group, kRows));
+  const unsigned long long bound = attn_tiles(a.rows_q, a.max_q, a.seqs, a.group, kRows, &a.q_each);
+  if (bound >= 1ull << 31) return B200_ERR_TOO_LARGE;
+  const uint32_t tiles = static_cast<uint32_t>(bound);
   auto kernel = attention_fw_kernel<T, kD, kPass>;
   if (const int rc = allow_smem(kernel, smem)) return rc;
   const uint32_t splits = split_of(ctx, static_cast<unsigned long long>(tiles) * a.heads_k, a.max_k / kFwCols<T, kD>);
@@ -426,10 +428,12 @@ int launch_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
 }
 
 template <typename T, int kD, int kPass>
-int launch_bw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
+int launch_bw(b200_ctx *ctx, AttnArgs a, cudaStream_t s) {
   constexpr size_t smem = sizeof(T) * kPitch<T, kD> * (2 * kRows + 2 * kBwStages<T, kD> * kBwCols<T, kD>);
-  const uint32_t k_tiles = static_cast<uint32_t>(attn_tile_bound(a.rows_k, a.max_k, a.seqs, 1, kRows));
-  const uint32_t q_tiles = static_cast<uint32_t>(attn_tile_bound(a.rows_q, a.max_q, a.seqs, a.group, kRows));
+  const unsigned long long k_bound = attn_tiles(a.rows_k, a.max_k, a.seqs, 1, kRows, &a.k_each);
+  const unsigned long long q_bound = attn_tiles(a.rows_q, a.max_q, a.seqs, a.group, kRows, &a.q_each);
+  if (k_bound + q_bound >= 1ull << 31) return B200_ERR_TOO_LARGE;
+  const uint32_t k_tiles = static_cast<uint32_t>(k_bound), q_tiles = static_cast<uint32_t>(q_bound);
   if (k_tiles + q_tiles == 0) return B200_OK;
   auto kernel = attention_bw_kernel<T, kD, kPass>;
   if (const int rc = allow_smem(kernel, smem)) return rc;

@@ -960,7 +960,7 @@ int attention_tc_fw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
   p.a = a;
   p.two_heads = a.group % 2 == 0;
   p.columns = p.two_heads ? a.heads_q / 2 : a.heads_q;
-  const unsigned long long tiles = attn_tile_bound(a.rows_q, a.max_q, a.seqs, 1, p.two_heads ? kTile : 2 * kTile);
+  const unsigned long long tiles = attn_tiles(a.rows_q, a.max_q, a.seqs, 1, p.two_heads ? kTile : 2 * kTile, &p.a.q_each);
   if (tiles * p.columns > 0x7fffffffull) return B200_ERR_TOO_LARGE;
   p.tiles = static_cast<uint32_t>(tiles);
   p.status = ctx->d_status;
@@ -986,7 +986,7 @@ int attention_tc_bw(b200_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
   if (rc == B200_OK) rc = encode(ctx, &p.v, a.v, a.head, a.heads_k, a.rows_k, a.v_ld);
   if (rc == B200_OK) rc = encode(ctx, &p.gy, a.gy, a.head, a.heads_q, a.rows_q, a.y_ld);
   if (rc != B200_OK) return rc;
-  const unsigned long long k_tiles = attn_tile_bound(a.rows_k, a.max_k, a.seqs, 1, kTile), q_tiles = attn_tile_bound(a.rows_q, a.max_q, a.seqs, 1, kTile);
+  const unsigned long long k_tiles = attn_tiles(a.rows_k, a.max_k, a.seqs, 1, kTile, &p.a.k_each), q_tiles = attn_tiles(a.rows_q, a.max_q, a.seqs, 1, kTile, &p.a.q_each);
   const unsigned long long blocks = k_tiles * a.heads_k + q_tiles * a.heads_q;
   if (blocks > 0x7fffffffull) return B200_ERR_TOO_LARGE;
   if (blocks == 0) return B200_OK;

@@ -509,7 +509,7 @@ int check(RotaryArgs *a, int layout, bool norm) {
   if (layout != B200_ROTARY_PAIRS && layout != B200_ROTARY_HALVES) return B200_ERR_INVALID_ARG;
   if (a->head == 0 || a->rot > a->head || a->rot % 2 != 0 || (a->rot != 0 && !a->freqs)) return B200_ERR_INVALID_ARG;
   if (a->head > kMaxHead) return B200_ERR_TOO_LARGE;
-  if (static_cast<u64>(a->heads) * a->head > 0x7fffffffu) return B200_ERR_TOO_LARGE;
+  if (static_cast<u64>(a->heads) * a->head > 0x7fffffffu || a->tokens > 0x7fffffffu) return B200_ERR_TOO_LARGE;
   const u64 dense = static_cast<u64>(a->heads) * a->head;
   for (u64 *ld : {&a->x_ld, &a->g_ld, &a->y_ld}) {
     if (*ld == 0) *ld = dense;

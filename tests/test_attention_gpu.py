@@ -245,6 +245,42 @@ def test_more_sequences_than_a_step_of_the_search(ctx):
     p.check()
 
 
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32"])
+@pytest.mark.parametrize("longest", [70, 300])
+def test_thousands_of_sequences(ctx, mode, longest):
+    """One long sequence among 3000 short ones: tiles are numbered through all of them, or apart for each."""
+    lengths = [(i * 7) % 4 for i in range(3000)]
+    lengths[1234] = longest
+    at = packed(lengths)
+    p = Problem(mode, 64, 2, 1, at, at, True, seed=25)
+    p.forward(ctx)
+    p.backward(ctx)
+    # a few of them: each is compared on its own
+    some = [0, 1, 2, 3, 1233, 1234, 1235, 2998, 2999]
+    group = Problem(mode, 64, 2, 1, packed([1]), packed([1]), True, seed=26)
+    for n in ("q", "k", "v", "gy"):
+        setattr(group, n, torch.cat([getattr(p, n)[at[i][0]:at[i][0] + at[i][1]] for i in some]))
+    group.q_at = group.k_at = packed([at[i][1] for i in some])
+    group.rows_q = group.rows_k = group.q.shape[0]
+    group.y = torch.cat([p.y[at[i][0]:at[i][0] + at[i][1]] for i in some])
+    group.lse = torch.cat([p.lse[:, at[i][0]:at[i][0] + at[i][1]] for i in some], 1)
+    for n in ("gq", "gk", "gv"):
+        setattr(group, n, torch.cat([getattr(p, n)[at[i][0]:at[i][0] + at[i][1]] for i in some]))
+    group.check(gradients=True)
+    assert not any(g.isnan().any() for g in (p.y, p.gq, p.gk, p.gv))
+
+
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32"])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+@pytest.mark.parametrize("tokens", [1, 130])
+def test_scales_that_are_not_positive(ctx, mode, scale, tokens):
+    q_at = packed([tokens, tokens])
+    p = Problem(mode, 64, 4, 2, q_at, packed([140, 150]), True, seed=27, scale=scale)
+    p.forward(ctx)
+    p.backward(ctx)
+    p.check(gradients=True)
+
+
 def test_starts_beyond_the_rows_are_cut(ctx):
     """Numbers that a faulty program could hold: nothing outside the arrays is read or written."""
     at = [(0, 40), (40, 24)]

@@ -217,3 +217,22 @@ def test_refusals(ctx):
             call()
         assert e.value.code == code
     ctx.norm_rotary_fw(0, X, G, None, Y, 8, 2, 0, 4, 0, 0, 8, 0, F)      # no heads of keys: no gain for them
+
+
+def test_heads_of_either_kind_may_be_missing(ctx):
+    """All heads as queries, or all as keys: the same numbers, and the other gain's gradient is nothing."""
+    t, h, d = 333, 5, 96
+    gen = torch.Generator(device="cuda").manual_seed(30)
+    x, gy = (torch.randn(t, h, d, device="cuda", generator=gen).half() for _ in range(2))
+    gain = (1 + 0.1 * torch.randn(d, device="cuda", generator=gen)).half()
+    f = torch.tensor(pb.rotary_frequencies(d)[0], device="cuda", dtype=torch.float64)
+    scratch, runs = torch.empty(pb.NORM_ROTARY_SCRATCH, device="cuda"), []
+    for hq, hk in ((h, 0), (0, h)):
+        y, gx, gg = torch.empty_like(x), torch.empty_like(x), torch.full((2, d), 9.0, device="cuda").half()
+        gains = (gain.data_ptr(), None) if hq else (None, gain.data_ptr())
+        ctx.norm_rotary_fw(2, x.data_ptr(), *gains, y.data_ptr(), d, hq, hk, t, 0, 0, d, PAIRS, f.data_ptr())
+        ctx.norm_rotary_bw(2, x.data_ptr(), *gains, gy.data_ptr(), gx.data_ptr(), gg[0].data_ptr(), gg[1].data_ptr(), scratch.data_ptr(), d, hq, hk, t,
+                           0, 0, 0, d, PAIRS, f.data_ptr(), accumulate_x=False, accumulate_gain=False)
+        runs.append((y, gx, gg[0] if hq else gg[1]))
+        assert ((gg[1] if hq else gg[0]) == 0).all()
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
