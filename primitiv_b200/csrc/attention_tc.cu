@@ -478,7 +478,7 @@ constexpr float kPBits = 13.f;
 template <int kD> constexpr uint32_t kY1 = kD == 128 ? 3u : 4u;
 template <int kD> constexpr uint32_t kY2 = kD == 128 ? 2u : 3u;
 constexpr uint32_t kStats = 2;
-constexpr uint32_t kBwHead = 3072;   // bytes in front of the tiles; with 7 tiles of 32 KB that is all there is
+constexpr uint32_t kBwHead = 3 * 1024;   // bytes in front of the tiles; with 7 tiles of 32 KB that is all there is
 template <int kD> constexpr uint32_t kBwSmem = kBwHead + (2 + kY1<kD> + kY2<kD>) * kTile * kD * 2;
 
 struct BwShared {
