@@ -64,19 +64,19 @@ __device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, u
   if constexpr (kD == 64) asm volatile(B200_NT_HEAD B200_NT_FOUR("f") "}\n" B200_NT_ARGS);
   else asm volatile(B200_NT_HEAD B200_NT_FOUR("f") "add.u64 da, da, 1018; add.u64 db, db, 1018;\n\t" B200_NT_FOUR("t") "}\n" B200_NT_ARGS);
 }
-// d[128][N] (+)= P . B, P of 128 halves a row in tensor memory, B a tile of 128 rows in chunks of 64 columns.  kGap: p lies in two runs of
-// 32 columns, 64 apart.
-#define B200_PN(MIDDLE) \
+// d[128][N] (+)= P . B, P of 128 halves a row in tensor memory, B a tile of 128 rows in chunks of 64 columns.  kGap: p lies in runs of
+// 16 columns, 32 apart.
+#define B200_PN(EVEN) \
   "{\n\t.reg .pred e, t, f;\n\t.reg .b32 a;\n\t.reg .b64 db;\n\t" \
   "setp.ne.b32 e, %5, 0; setp.eq.b32 t, %3, %3; setp.ne.b32 f, %6, 0;\n\tmov.b32 a, %1; mov.b64 db, {%2, %3};\n\t" \
-  B200_MMA_TS "f;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" \
-  B200_NEXT_TS(MIDDLE) B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") \
+  B200_MMA_TS "f;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS(EVEN) B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" \
+  B200_NEXT_TS(EVEN) B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") B200_MMA_TS "t;\n\t" B200_NEXT_TS(EVEN) B200_MMA_TS "t;\n\t" B200_NEXT_TS("8") \
   B200_MMA_TS "t;\n\t}\n"
 #define B200_PN_ARGS \
   ::"r"(d), "r"(p), "r"(((b & 0x3FFFFu) >> 4) | ((kChunk >> 4) << 16)), "r"(kDescHi), "r"(idesc), "r"(leader), "r"(first ? 0u : 1u) : "memory"
 template <bool kGap = false>
 __device__ __forceinline__ void product_pn(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first, uint32_t leader) {
-  if constexpr (kGap) asm volatile(B200_PN("40") B200_PN_ARGS);
+  if constexpr (kGap) asm volatile(B200_PN("24") B200_PN_ARGS);
   else asm volatile(B200_PN("8") B200_PN_ARGS);
 }
 // Arrives on `bar` when every product issued so far is done.
@@ -97,6 +97,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -161,7 +168,7 @@ __device__ __forceinline__ void exp2_by_products(f32x2 x, float &u, float &w) {
 }
 // Of eight pairs, kByProducts go that way: the special function units of an SM do 16 elements a clock, as many as its tensor core needs of
 // them at full rate.  More of them cost more instructions than they save: a warp is alone on its scheduler for most of its softmax.
-// (0, 1, 2, 3 of 8: 1.84, 1.82, 1.86, 1.88 ms for the 16384 tokens above.)
+// (0, 1, 2 of 8: 1.84, 1.82, 1.86 ms for the 16384 tokens above.)
 constexpr int kByProducts = 1;
 __device__ __forceinline__ void exp2_pair(int nth, f32x2 x, float &u, float &w) {
   if ((nth & 7) < kByProducts) {
@@ -452,8 +459,9 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
 //   keys at rest     X1 = k, X2 = v, Y1 = q, Y2 = gy:   s' = k q^T, dp' = v gy^T,  gv += p' gy,  gk += ds' q
 //   queries at rest  X1 = q, X2 = gy, Y1 = k, Y2 = v:   s = q k^T,  dp = gy v^T,   gq += ds k
 // Transposed where the keys rest, so that p and ds are always the left operand, from tensor memory, and a tile in shared memory
-// serves both as the right operand of the first products and of the second.  Eight warps share a tile: a thread has 64 of a
-// row's 128 columns.
+// serves both as the right operand of the first products and of the second.  Sixteen warps share a tile: a thread has 32 of a
+// row's 128 columns.  Four warps on a scheduler fill one another's waits, and 96 registers are enough without moving any.  (6 packed sequences of up to 4096 tokens, 16 heads of 128 on 4,
+// forward and backward: 794 us with eight warps of 64 columns a thread, 753 with sixteen.)
 //   keys at rest: the sums take half of tensor memory, so s and dp have one place between them: s(i) is in registers when dp(i) is
 //     issued, and dp(i) is when s(i+1) is.  Order of the products: dp(i) s(i+1) gv(i), dp(i+1) gk(i) ...
 //     (With places of their own, p written over s and ds over dp, s(i+1) waited for gv(i) and that for p(i): 3250 clocks a step.)
@@ -471,7 +479,8 @@ struct alignas(64) BwParams {
   int *status;
 };
 
-constexpr uint32_t kBwThreads = 384;
+constexpr uint32_t kBwWarps = 16;                       // for p and ds; four more for products, copies and preparing tiles
+constexpr uint32_t kBwThreads = (4 + kBwWarps) * 32;
 constexpr float kPBits = 13.f;
 // Slots of the rings.  Y1 is needed first and given back last, by the product that ends a step: with two slots its copy started a step
 // late, and a step with queries at rest took 3500 clocks instead of 1900.
@@ -528,7 +537,7 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
     for (uint64_t *one : {&sh.x_full, &sh.s_full, &sh.dp_full[0], &sh.dp_full[1], &sh.acc_done, &sh.drain}) mbar_init(smem_u32(one), 1);
     for (uint32_t i = 0; i < 4; ++i)
       for (uint64_t *one : {&sh.full1[i], &sh.ready1[i], &sh.empty1[i], &sh.full2[i], &sh.ready2[i], &sh.empty2[i]}) mbar_init(smem_u32(one), 1);
-    for (uint64_t *warps : {&sh.s_read, &sh.dp_read, &sh.p_full, &sh.ds_full[0], &sh.ds_full[1]}) mbar_init(smem_u32(warps), 8);
+    for (uint64_t *warps : {&sh.s_read, &sh.dp_read, &sh.p_full, &sh.ds_full[0], &sh.ds_full[1]}) mbar_init(smem_u32(warps), kBwWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
@@ -596,8 +605,6 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
       ds_scale = scale_of(gm, vm, dm);
     }
 
-    // 168 registers a thread at launch: 56 + 2 * 224 = 3 * 168
-    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 1) {
       // ------------------------------ copies ------------------------------
       if (steps > 0) {
@@ -743,8 +750,7 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
       }
     } else if (warp >= 4) {
       // ------------------------------ p and ds ------------------------------
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-      const uint32_t half = (warp >> 2) - 1u, quarter = warp & 3u, col0 = half * 64u;
+      const uint32_t part = (warp >> 2) - 1u, quarter = warp & 3u, col0 = part * 32u;   // a thread has 32 of a row's 128 columns
       const uint32_t lanes = (quarter * 32u) << 16, s_tmem = tmem + lanes + col0;
       const uint32_t row = row0 + quarter * 32u + lane;
       const float to2 = a.scale * kLog2e;
@@ -771,83 +777,71 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
         if (kKeys && !wait_all(smem_u32(&sh.ready1[s1.at]), s1.phase, abort_flag)) { ok = false; break; }
         if (!wait_all(smem_u32(&sh.s_full), i & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        uint32_t s[2][32];
-        tmem_ld32_issue(s_tmem, s[0]);
-        tmem_ld32_issue(s_tmem + 32, s[1]);
-        tmem_ld_wait(s[0]);
-        tmem_ld_wait(s[1]);
+        uint32_t s[32];
+        tmem_ld32(s_tmem, s);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.s_read));
-        // columns of this thread that its row has no part in: [0, skip) where queries pass by, [skip, 64) where keys do
+        // columns of this thread that its row has no part in: [0, skip) where queries pass by, [skip, 32) where keys do
         int skip;
         if constexpr (kKeys) {
           const long long first = a.causal ? static_cast<long long>(row) - shift - (from + static_cast<long long>(t) * kTile) - col0 : 0ll;
-          skip = static_cast<int>(max(0ll, min(first, 64ll)));
+          skip = static_cast<int>(max(0ll, min(first, 32ll)));
         } else {
-          skip = static_cast<int>(max(0ll, min(sees - static_cast<long long>(i) * kTile - col0, 64ll)));
+          skip = static_cast<int>(max(0ll, min(sees - static_cast<long long>(i) * kTile - col0, 32ll)));
         }
-        if (__any_sync(0xffffffffu, kKeys ? skip > 0 : skip < 64)) {
+        if (__any_sync(0xffffffffu, kKeys ? skip > 0 : skip < 32)) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (kKeys ? c * 32 + e < skip : c * 32 + e >= skip) s[c][e] = 0xff800000u;
+          for (int e = 0; e < 32; ++e)
+            if (kKeys ? e < skip : e >= skip) s[e] = 0xff800000u;
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int e = 0; e < 32; e += 4) {
+          f32x2 add[2] = {base2, base2};
+          if constexpr (kKeys) stat4(stat0 + e, add[0], add[1]);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            f32x2 add[2] = {base2, base2};
-            if constexpr (kKeys) stat4(stat0 + c * 32 + e, add[0], add[1]);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int at = e + 2 * k;
-              float u, w;
-              exp2_pair(at / 2, fma2(pair_of(__uint_as_float(s[c][at]), __uint_as_float(s[c][at + 1])), to22, add[k]), u, w);
-              s[c][at] = __float_as_uint(u), s[c][at + 1] = __float_as_uint(w);
-            }
+          for (int k = 0; k < 2; ++k) {
+            const int at = e + 2 * k;
+            float u, w;
+            exp2_pair(at / 2, fma2(pair_of(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), to22, add[k]), u, w);
+            s[at] = __float_as_uint(u), s[at + 1] = __float_as_uint(w);
           }
+        }
         if (!wait_all(smem_u32(&sh.dp_full[kKeys ? 0u : b]), (kKeys ? i : i >> 1) & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        uint32_t d[2][32], out[32];
-        tmem_ld32_issue(dp_tmem, d[0]);
-        tmem_ld32_issue(dp_tmem + 32, d[1]);
-        tmem_ld_wait(d[0]);
-        tmem_ld_wait(d[1]);
+        uint32_t d[32], out[16];
+        tmem_ld32(dp_tmem, d);
         if constexpr (kKeys) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sh.dp_read));
           // (dp(i) is issued behind gv(i - 1), so p(i - 1) is read)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) out[e] = halves_of(__uint_as_float(s[e >> 4][(e & 15) * 2]), __uint_as_float(s[e >> 4][(e & 15) * 2 + 1]));
-          tmem_st32(tmem + lanes + kP + half * 32u, out);
+          for (int e = 0; e < 16; ++e) out[e] = halves_of(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+          tmem_st16(tmem + lanes + kP + part * 16u, out);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int e = 0; e < 32; e += 4) {
+          f32x2 add[2] = {minus_delta2, minus_delta2};
+          if constexpr (kKeys) stat4(stat1 + e, add[0], add[1]);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            f32x2 add[2] = {minus_delta2, minus_delta2};
-            if constexpr (kKeys) stat4(stat1 + c * 32 + e, add[0], add[1]);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int at = e + 2 * k;
-              float u, w;
-              unpair(mul2(pair_of(__uint_as_float(s[c][at]), __uint_as_float(s[c][at + 1])),
-                          fma2(pair_of(__uint_as_float(d[c][at]), __uint_as_float(d[c][at + 1])), f2, add[k])), u, w);
-              out[c * 16 + at / 2] = halves_of(u, w);
-            }
+          for (int k = 0; k < 2; ++k) {
+            const int at = e + 2 * k;
+            float u, w;
+            unpair(mul2(pair_of(__uint_as_float(s[at]), __uint_as_float(s[at + 1])),
+                        fma2(pair_of(__uint_as_float(d[at]), __uint_as_float(d[at + 1])), f2, add[k])), u, w);
+            out[at / 2] = halves_of(u, w);
           }
+        }
         if constexpr (kKeys) {   // gk(i - 1) has read its ds
           if (i > 0 && !wait_all(smem_u32(&sh.empty1[(i - 1) % kSlots1]), ((i - 1) / kSlots1) & 1u, abort_flag)) { ok = false; break; }
           tc_fence_after();
         }
-        tmem_st32(kKeys ? tmem + lanes + kDs + half * 32u : dp_tmem, out);
+        tmem_st16(kKeys ? tmem + lanes + kDs + part * 16u : dp_tmem, out);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -858,23 +852,25 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
       if (ok && steps > 0) ok = wait_all(smem_u32(&sh.acc_done), 0, abort_flag);
       tc_fence_after();
       if (ok) {
-        // keys at rest: gv by the first four warps, gk by the others; queries at rest: half of gq's columns each
-        const float undo = kKeys && half == 0 ? exp2f(-kPBits) : a.scale / ds_scale;
-        constexpr int kCols = kKeys ? kD : kD / 2;
-        const uint32_t c0 = kKeys ? 0u : half * kCols;
-        const uint32_t acc = tmem + lanes + (kKeys && half == 0 ? kAcc1 : kAcc2) + c0;
+        // keys at rest: half of gv's columns by either of the first two fours of warps, of gk's by the others; queries at rest: a quarter
+        // of gq's columns each
+        const bool is_v = kKeys && part < 2u;
+        const float undo = is_v ? exp2f(-kPBits) : a.scale / ds_scale;
+        constexpr int kCols = kKeys ? kD / 2 : kD / 4;
+        const uint32_t c0 = (kKeys ? part & 1u : part) * kCols;
+        const uint32_t acc = tmem + lanes + (is_v ? kAcc1 : kAcc2) + c0;
         __half *out;
         if constexpr (kKeys)
-          out = half == 0 ? static_cast<__half *>(a.gv) + (q.k0 + static_cast<unsigned long long>(row)) * a.v_ld + static_cast<unsigned long long>(kv_head) * a.head
-                          : static_cast<__half *>(a.gk) + (q.k0 + static_cast<unsigned long long>(row)) * a.k_ld + static_cast<unsigned long long>(kv_head) * a.head;
+          out = is_v ? static_cast<__half *>(a.gv) + (q.k0 + static_cast<unsigned long long>(row)) * a.v_ld + static_cast<unsigned long long>(kv_head) * a.head
+                     : static_cast<__half *>(a.gk) + (q.k0 + static_cast<unsigned long long>(row)) * a.k_ld + static_cast<unsigned long long>(kv_head) * a.head;
         else
           out = static_cast<__half *>(a.gq) + (q.q0 + static_cast<unsigned long long>(row)) * a.q_ld + static_cast<unsigned long long>(q_head) * a.head;
 #pragma unroll
-        for (int c = 0; c < kCols; c += 32) {
-          uint32_t y[32];
-          if (steps > 0) tmem_ld32(acc + c, y);
+        for (int c = 0; c < kCols; c += 16) {
+          uint32_t y[16];
+          if (steps > 0) tmem_ld16(acc + c, y);
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
+          for (int e = 0; e < 16; e += 8) {
             if (row < rows && c0 + c + e < a.head) {
               float v[8];
 #pragma unroll
