@@ -195,7 +195,9 @@ struct alignas(64) FwParams {
   int *status;
 };
 
-constexpr uint32_t kFwThreads = 384;   // three warps on each quarter of an SM; two of the first four only lend their registers
+// Three warps on each quarter of an SM; two of the first four only lend their registers.  (16384 tokens, 32 heads of 128 on 8: 1812 us; with
+// two threads a row, as the gradients have them, 2030, for what they have to tell one another; with p handed over in halves 1843.)
+constexpr uint32_t kFwThreads = 384;
 // Slots for tiles of keys and of values.
 template <int kD> constexpr uint32_t kFwK = kD == 128 ? 2u : 4u;
 template <int kD> constexpr uint32_t kFwV = kD == 128 ? 3u : 4u;
