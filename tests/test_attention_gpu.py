@@ -487,3 +487,59 @@ def test_nans_are_not_lost(ctx, mode, rows):
             assert not p.y[torch.arange(200, device="cuda") != column].isnan().any()
             p.backward(ctx)
             assert p.gq[column, 1].isnan().all() and not p.gq[:, 0].isnan().any() and p.gv[:column + 1].isnan().all()
+
+
+@pytest.mark.parametrize("head", [8, 16, 24, 48, 104, 120])
+def test_halves_of_short_heads(ctx, head):
+    at = packed([150, 66], first=1)
+    p = Problem("fp16", head, 4, 2, at, at, True, seed=head)
+    p.forward(ctx)
+    p.backward(ctx)
+    p.check(gradients=True)
+
+
+@pytest.mark.parametrize("head", [64, 17])
+@pytest.mark.parametrize("queries", [1, 130])
+def test_offsets_that_pass_32_bits(ctx, head, queries):
+    """Keys, values and their gradients in rows of a megabyte and more: the same bits as from rows of their own."""
+    ld, at = (1 << 20) + 8, packed([100, 4300])
+    p = Problem("fp16", head, 2, 2, packed([queries, queries]), at, True, seed=41)
+    p.forward(ctx)
+    p.backward(ctx)
+    p.check(gradients=True)
+    want = [t.clone() for t in (p.y, p.lse, p.gq, p.gk, p.gv)]
+    far = [torch.empty(p.rows_k * ld, device="cuda", dtype=p.dtype) for _ in range(2)]
+    assert far[0].numel() > 1 << 32
+    k, v, gk, gv = (f[2 * head * i:].as_strided((p.rows_k, 2, head), (ld, head, 1)) for f in far for i in range(2))
+    k.copy_(p.k), v.copy_(p.v), gk.fill_(NAN), gv.fill_(NAN)
+    p.k, p.v = k, v
+    p.y.fill_(7.0), p.lse.fill_(7.0), p.gq.fill_(NAN)
+    plan = p.plan()
+    p.forward(ctx, plan)
+    ctx.attention_bw(p.mode, plan, p.q.data_ptr(), k.data_ptr(), v.data_ptr(), p.y.data_ptr(), p.lse.data_ptr(), p.gy.data_ptr(), p.gq.data_ptr(),
+                     gk.data_ptr(), gv.data_ptr(), p.scratch.data_ptr(), accumulate=False)
+    assert all(torch.equal(a, b) for a, b in zip((p.y, p.lse, p.gq, gk, gv), want))
+
+
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32"])
+def test_two_calls_at_once(ctx, mode):
+    """On two streams, each with its own outputs and scratch: the bits that either call gives alone."""
+    problems = [Problem(mode, 64, 4, 2, packed(n), packed(n), True, seed=len(n)) for n in ([700, 90, 300], [1, 555, 40, 260])]
+    plans, want = [p.plan() for p in problems], []
+    for p, plan in zip(problems, plans):
+        p.forward(ctx, plan)
+        p.backward(ctx, plan)
+        want.append([t.clone() for t in (p.y, p.lse, p.gq, p.gk, p.gv)])
+    streams = [torch.cuda.Stream() for _ in problems]
+    for p in problems:
+        for t in (p.y, p.lse, p.gq, p.gk, p.gv):
+            t.fill_(NAN)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for p, plan, s in zip(problems, plans, streams):
+            p.forward(ctx, plan, stream=s.cuda_stream)
+            ctx.attention_bw(p.mode, plan, p.q.data_ptr(), p.k.data_ptr(), p.v.data_ptr(), p.y.data_ptr(), p.lse.data_ptr(), p.gy.data_ptr(),
+                             p.gq.data_ptr(), p.gk.data_ptr(), p.gv.data_ptr(), p.scratch.data_ptr(), accumulate=False, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for p, w in zip(problems, want):
+        assert all(torch.equal(a, b) for a, b in zip((p.y, p.lse, p.gq, p.gk, p.gv), w))

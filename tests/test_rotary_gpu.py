@@ -236,3 +236,32 @@ def test_heads_of_either_kind_may_be_missing(ctx):
         runs.append((y, gx, gg[0] if hq else gg[1]))
         assert ((gg[1] if hq else gg[0]) == 0).all()
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_offsets_that_pass_32_bits(ctx):
+    """Tokens in rows of a megabyte and more, forward and backward: the same bits as from rows of their own."""
+    t, h, d, ld = 4200, 3, 64, (1 << 20) + 8
+    f = torch.tensor(pb.rotary_frequencies(d)[0], device="cuda", dtype=torch.float64)
+    near = [inputs((t, h, d), torch.float16, seed)[0] for seed in (51, 52)]
+    gains = (1 + 0.3 * torch.randn(2, d, device="cuda")).half()
+    buffers = [torch.empty(t * ld, device="cuda", dtype=torch.float16) for _ in range(3)]
+    assert buffers[0].numel() > 1 << 32
+    far = [b.as_strided((t, h, d), (ld, d, 1)) for b in buffers]
+    for a, b in zip(far, near):
+        a.copy_(b)
+    scratch = torch.empty(pb.NORM_ROTARY_SCRATCH, device="cuda")
+    code, eps = MODES["fp16"][0], 1e-5
+
+    def every(x, gy, out, at):
+        got = []
+        keep = lambda: got.append(out.contiguous().clone())
+        ctx.rotary_fw(code, x.data_ptr(), out.data_ptr(), d, h, t, at, at, d, HALVES, f.data_ptr()), keep()
+        ctx.rotary_bw(code, gy.data_ptr(), out.data_ptr(), d, h, t, at, at, d, PAIRS, f.data_ptr(), accumulate=False), keep()
+        more = (d, HALVES, f.data_ptr(), 1.0, None, eps)
+        ctx.norm_rotary_fw(code, x.data_ptr(), gains[0].data_ptr(), gains[1].data_ptr(), out.data_ptr(), d, 2, 1, t, at, at, *more), keep()
+        sums = torch.zeros_like(gains)
+        ctx.norm_rotary_bw(code, x.data_ptr(), gains[0].data_ptr(), gains[1].data_ptr(), gy.data_ptr(), out.data_ptr(), sums[0].data_ptr(),
+                           sums[1].data_ptr(), scratch.data_ptr(), d, 2, 1, t, at, at, at, *more, accumulate_x=False), keep()
+        return got + [sums]
+    want = every(near[0], near[1], torch.zeros_like(near[0]), h * d)
+    assert all(torch.equal(a, b) for a, b in zip(every(*far, ld), want))
