@@ -167,6 +167,15 @@ __device__ __forceinline__ void load_raw(Raw<T, V> &raw, const T *p, uint32_t c0
   if (c0 < head) raw.first = *reinterpret_cast<const Pack<T, V> *>(p + c0);
   if (c1 < head) raw.second = *reinterpret_cast<const Pack<T, V> *>(p + c1);
 }
+// The same element by element, from any address.
+template <typename T, int V>
+__device__ __forceinline__ void load_raw_any(Raw<T, V> &raw, const T *p, uint32_t c0, uint32_t c1, uint32_t head) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (c0 < head) raw.first.v[j] = p[c0 + j];
+    if (c1 < head) raw.second.v[j] = p[c1 + j];
+  }
+}
 // What there is none of counts as zero.
 template <typename T, int V, int kLayout>
 __device__ __forceinline__ Unit<V> unit_of(const Raw<T, V> &raw, bool has0, bool has1) {
@@ -254,7 +263,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
       Raw<T, V> raw;
-      load_raw(raw, static_cast<const T *>(second ? a.gain_k : a.gain_q), c0[k], c1[k], a.head);
+      // (once in a block, so it need not be in vectors, and gains may begin at any element of a buffer of parameters)
+      load_raw_any(raw, static_cast<const T *>(second ? a.gain_k : a.gain_q), c0[k], c1[k], a.head);
       gain[k] = unit_of<T, V, kLayout>(raw, c0[k] < a.head, c1[k] < a.head);
       if constexpr (kSums) sums[k].a = sums[k].b = all_of<V>(0.f);
     }

@@ -265,3 +265,30 @@ def test_offsets_that_pass_32_bits(ctx):
         return got + [sums]
     want = every(near[0], near[1], torch.zeros_like(near[0]), h * d)
     assert all(torch.equal(a, b) for a, b in zip(every(*far, ld), want))
+
+
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32"])
+@pytest.mark.parametrize("head, rot, layout", [(64, 64, HALVES), (128, 32, PAIRS), (96, 96, HALVES), (34, 12, PAIRS), (33, 6, HALVES)])
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_gains_off_every_boundary(ctx, mode, head, rot, layout, shift):
+    """Gains that start anywhere in a buffer of parameters, beside x, y and gy on 16-byte boundaries: the bits that aligned gains give."""
+    t, hq, hk = 37, 3, 2
+    code, dtype = MODES[mode][:2]
+    (x, _), (gy, _) = (inputs((t, hq + hk, head), dtype, seed) for seed in (71, 72))
+    f = torch.tensor(pb.rotary_frequencies(rot)[0], device="cuda", dtype=torch.float64)
+    aligned = [(1 + 0.3 * torch.randn(head, device="cuda")).to(dtype) for _ in range(2)]
+    sums = torch.full((2 * head + 8,), 9.0, device="cuda", dtype=dtype)
+    params = torch.full((2 * head + 8,), float("nan"), device="cuda", dtype=dtype)
+    shifted = [params[shift:shift + head], params[shift + head + 1:shift + 2 * head + 1]]
+    for a, b in zip(shifted, aligned):
+        a.copy_(b)
+    scratch, runs = torch.empty(pb.NORM_ROTARY_SCRATCH, device="cuda"), []
+    for gains, gg in ((aligned, [torch.empty_like(a) for a in aligned]), (shifted, [sums[shift:shift + head], sums[shift + head + 1:shift + 2 * head + 1]])):
+        y, gx = torch.empty_like(x), torch.empty_like(x)
+        at, more = [g.data_ptr() for g in gains], (rot, layout, f.data_ptr())
+        ctx.norm_rotary_fw(code, x.data_ptr(), *at, y.data_ptr(), head, hq, hk, t, 0, 0, *more)
+        ctx.norm_rotary_bw(code, x.data_ptr(), *at, gy.data_ptr(), gx.data_ptr(), gg[0].data_ptr(), gg[1].data_ptr(), scratch.data_ptr(), head, hq, hk,
+                           t, 0, 0, 0, *more, accumulate_x=False, accumulate_gain=False)
+        runs.append([y, gx] + [g.clone() for g in gg])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    assert (sums[:shift] == 9.0).all() and sums[shift + head] == 9.0 and (sums[shift + 2 * head + 1:] == 9.0).all()
