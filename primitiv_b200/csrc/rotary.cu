@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
         }
         float ss = sum_of(sq), dot = kBack ? sum_of(dots) : 0.f;
         group_sums(ss, dot, a.lanes_log2);
-        const float rs = rsqrtf(ss * per_head + a.eps);
+        const float rs = here ? rsqrtf(ss * per_head + a.eps) : 0.f;   // (without a row, eps = 0 would make it infinite, and 0 * rs a NaN in the sums)
         const Lane<V> rs_all = all_of<V>(rs);
         if constexpr (!kBack) {
 #pragma unroll

@@ -292,3 +292,21 @@ def test_gains_off_every_boundary(ctx, mode, head, rot, layout, shift):
         runs.append([y, gx] + [g.clone() for g in gg])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
     assert (sums[:shift] == 9.0).all() and sums[shift + head] == 9.0 and (sums[shift + 2 * head + 1:] == 9.0).all()
+
+
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32"])
+@pytest.mark.parametrize("t, hq, hk, d, rot", [(1, 1, 1, 64, 64), (5, 3, 2, 64, 32), (67, 9, 1, 33, 6), (131, 5, 3, 128, 128)])
+def test_an_epsilon_of_zero(ctx, mode, t, hq, hk, d, rot):
+    """Blocks whose last tokens or heads do not exist, where x = 0 makes no infinite 1 / sqrt(0): nothing of them is in the sums."""
+    code, dtype = MODES[mode][:2]
+    store, tiny = store_rounding(dtype)
+    (x, _), (gy, _) = (inputs((t, hq + hk, d), dtype, seed) for seed in (61, 62))
+    gain_q, gain_k = (1 + 0.3 * torch.randn(2, d, device="cuda")).to(dtype)
+    f = torch.tensor(pb.rotary_frequencies(rot)[0], device="cuda", dtype=torch.float64)
+    angles = torch.arange(t, device="cuda").double()[:, None] * f
+    gx, ggq, ggk, e_gx, e_q, e_k = norm_reference(x, gain_q, gain_k, hq, angles, 1.0, rot, PAIRS, 0.0, gy)
+    got, gg, scratch = torch.empty_like(gx).to(dtype), torch.empty(2, d, device="cuda", dtype=dtype), torch.empty(pb.NORM_ROTARY_SCRATCH, device="cuda")
+    ctx.norm_rotary_bw(code, x.data_ptr(), gain_q.data_ptr(), gain_k.data_ptr(), gy.data_ptr(), got.data_ptr(), gg[0].data_ptr(), gg[1].data_ptr(),
+                       scratch.data_ptr(), d, hq, hk, t, 0, 0, 0, rot, PAIRS, f.data_ptr(), eps=0.0, accumulate_x=False, accumulate_gain=False)
+    for value, exact, bound in ((got, gx, e_gx), (gg[0], ggq, e_q), (gg[1], ggk, e_k)):
+        assert (abs(value.double() - exact) <= bound + store * (abs(exact) + bound) + tiny).all()
