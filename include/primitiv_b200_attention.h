@@ -38,8 +38,10 @@ enum { B200_ROTARY_PAIRS = 0, B200_ROTARY_HALVES = 1 };
  *     BASE      PLAIN with base * factor^(rot/(rot - 2)): the slowest pair is interpolated by
  *               `factor`, the fastest not at all
  *     BY_PARTS  pairs that turn less than once in `original` positions as LINEAR, more than 32
- *               times as PLAIN, between the two a blend that is linear in p; amplitude
- *               1 + 0.1 ln(factor), 1 in the other forms
+ *               times as PLAIN, between the two a blend that is linear in p: the share of LINEAR is
+ *               (p - first) / (last - first) between 0 and 1, first = floor(pair(32)), last = ceil(pair(1)),
+ *               pair(n) = rot ln(original / (2 pi n)) / (2 ln base), whether or not there are such pairs;
+ *               amplitude 1 + 0.1 ln(factor), 1 in the other forms
  * `amplitude_host` may be NULL. */
 enum { B200_ROTARY_PLAIN = 0, B200_ROTARY_LINEAR, B200_ROTARY_BASE, B200_ROTARY_BY_PARTS };
 B200_API int b200_rotary_frequencies(uint32_t rot, double base, int scaling, double factor, double original,

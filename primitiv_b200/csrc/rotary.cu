@@ -550,17 +550,18 @@ int b200_rotary_frequencies(uint32_t rot, double base, int scaling, double facto
   double amplitude = 1.0, lo = 0.0, hi = 0.0;
   if (scaling == B200_ROTARY_BASE && rot > 2) base *= std::pow(factor, r / (r - 2.0));
   if (scaling == B200_ROTARY_BY_PARTS) {
-    // the pair that turns n times in `original` positions: original base^(-2p/rot) = 2 pi n
+    // the pair that turns n times in `original` positions: original base^(-2p/rot) = 2 pi n.  There need not be one: of a long context
+    // all pairs turn more than once, and the blend ends behind the last.
     auto pair = [&](double n) { return r * std::log(original / (n * pi2)) / (2.0 * std::log(base)); };
-    lo = std::max(std::floor(pair(32.0)), 0.0);
-    hi = std::min(std::ceil(pair(1.0)), r / 2.0 - 1.0);
+    lo = std::floor(pair(32.0));
+    hi = std::ceil(pair(1.0));
     amplitude = 1.0 + 0.1 * std::log(factor);
   }
   for (uint32_t p = 0; p < rot / 2; ++p) {
     double f = std::pow(base, -2.0 * p / r);
     if (scaling == B200_ROTARY_LINEAR) f /= factor;
     if (scaling == B200_ROTARY_BY_PARTS) {
-      const double slow = std::min(std::max((p - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+      const double slow = std::min(std::max((p - lo) / (hi - lo), 0.0), 1.0);
       f = f / factor * slow + f * (1.0 - slow);
     }
     freqs_host[p] = f;

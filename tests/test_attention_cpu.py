@@ -33,6 +33,41 @@ def test_scaled_frequencies():
             assert f / 4 * (1 - 1e-12) <= g <= f * (1 + 1e-12)
 
 
+def blend(rot, base, factor, original):
+    """By the definition: floor and ceiling of the pairs that turn 32 times and once, wherever those lie."""
+    at = [rot * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in (32.0, 1.0)]
+    first, last = math.floor(at[0]), math.ceil(at[1])
+    freqs = []
+    for p in range(rot // 2):
+        slow = min(max((p - first) / (last - first), 0.0), 1.0)
+        freqs.append(base ** (-2 * p / rot) * (1 - slow + slow / factor))
+    return freqs
+
+
+@pytest.mark.parametrize("rot, base, factor, original", [
+    (8, 1e4, 4.0, 8192.0), (128, 1e4, 4.0, 65536.0), (128, 1e4, 4.0, 131072.0), (64, 1e4, 8.0, 1e6), (2, 1e4, 4.0, 4096.0), (12, 5e5, 2.0, 1e9),
+    (64, 1e4, 4.0, 64.0), (64, 1e4, 4.0, 5.0), (128, 1e4, 8.0, 4096.0), (6, 10.0, 3.0, 1.0), (256, 1.5, 3.0, 1e30),
+])
+def test_blended_frequencies(rot, base, factor, original):
+    """The blend's ends may lie before the first pair and behind the last: pairs of long contexts all turn more than once."""
+    freqs, amplitude = pb.rotary_frequencies(rot, base, "by_parts", factor, original)
+    assert amplitude == pytest.approx(1 + 0.1 * math.log(factor), rel=1e-15)
+    assert freqs == pytest.approx(blend(rot, base, factor, original), rel=1e-14)
+    for p, f in enumerate(freqs):
+        plain = base ** (-2 * p / rot)
+        turns = original * plain / (2 * math.pi)
+        if turns < 1 - 1e-9:
+            assert f == pytest.approx(plain / factor, rel=1e-14)
+        elif turns > 32 + 1e-9:
+            assert f == pytest.approx(plain, rel=1e-14)
+
+
+def test_a_last_pair_that_turns_more_than_once_is_half_blended():
+    """8 elements, base 10000, 8192 positions: the last pair turns 1.3 times; the blend runs from pair 1 to pair 4."""
+    freqs, _ = pb.rotary_frequencies(8, 1e4, "by_parts", 4.0, 8192.0)
+    assert freqs == pytest.approx([1.0, 0.1, 0.01 * 0.75, 0.001 * 0.5], rel=1e-12)
+
+
 @pytest.mark.parametrize("args", [(0,), (7,), (8, 1.0), (8, math.nan), (8, 1e4, "linear", 0.5), (8, 1e4, "by_parts", 2.0, 0.0),
                                   (8, 1e4, "base", math.inf)])
 def test_refused_frequencies(args):
