@@ -88,7 +88,8 @@ B200_API int b200_norm_rotary_bw(b200_ctx *ctx, int mode, const void *x, const v
  * otherwise every query sees every key of its sequence.  A query that sees no key has y = 0,
  * lse = -infinity and no part in any gradient.  Keys, values and queries outside a sequence are never
  * used, whatever they hold.  Within a sequence a NaN or an infinity is not lost: it reaches every result
- * that depends on it.  (Where a product gives such a value the weight zero, behind the diagonal of a causal
+ * that depends on it, as a NaN or as what the formula makes of it: a query whose scores are all -infinity
+ * has lse = -infinity too, but NaNs in y.  (Where a product gives such a value the weight zero, behind the diagonal of a causal
  * sequence, it may reach further, as a NaN: one of v or gy, and in the gradients one of any input.)
  *
  * Sequence i has its queries in rows q_starts[i], q_starts[i] + 1, ... of q, y (and their

@@ -149,13 +149,13 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
         sum += w * ld_cluster(map_to_cta(smem_at(s_l + at), s));
         v[0] += w * o.x, v[1] += w * o.y, v[2] += w * o.z, v[3] += w * o.w;
       }
-      const bool any = top != -INFINITY;
       const uint32_t tok = rw / a.group, h = hk * a.group + rw - tok * a.group;
+      const bool sees = a.causal ? static_cast<long long>(tok) + shift >= 0 : q.lk > 0u;
       T *out = static_cast<T *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(h) * a.head + c;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < a.head) out[e] = round_to<T>(any ? v[e] / sum : v[e]);   // (a sum of zeros, or a NaN)
-      if (a.lse && c == 0) a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = any ? top * kLn2 + logf(sum) : sum - INFINITY;
+        if (c + e < a.head) out[e] = round_to<T>(sees ? v[e] / sum : v[e]);
+      if (a.lse && c == 0) a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = sees ? (top == -INFINITY ? 0.f : top * kLn2) + logf(sum) : -INFINITY;
     }
     cluster_sync_all();   // nobody leaves while another reads its part
     return;
@@ -165,10 +165,12 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
     l[r] = quad_sum(l[r]);
     if (row[r] >= rows) continue;
     const uint32_t tok = row[r] / a.group, h = hk * a.group + row[r] - tok * a.group;
-    const bool any = m[r] != -INFINITY;
+    // a row that sees no key has zeros, one that sees scores of -infinity alone 0 / 0; a maximum of -infinity also leaves out NaNs
+    const bool sees = last[r] >= 0;
     store_row<T, kD>(static_cast<T *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(h) * a.head, acc, r, 0, a.head,
-                     any ? 1.f / l[r] : 0.f, 0);
-    if (a.lse && t == 0) a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = any ? m[r] * kLn2 + logf(l[r]) : -INFINITY;
+                     sees ? 1.f / l[r] : 0.f, 0);
+    if (a.lse && t == 0)
+      a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = sees ? (m[r] == -INFINITY ? 0.f : m[r] * kLn2) + logf(l[r]) : -INFINITY;
   }
 }
 

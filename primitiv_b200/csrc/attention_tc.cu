@@ -417,8 +417,10 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
       if (ok && n > 0) ok = wait_all(smem_u32(&y_done[x]), (n - 1) & 1u, abort_flag);
       tc_fence_after();
       if (ok && x < count) {
-        const bool some = m != -INFINITY, mine = tok < q.lq;
-        const float inv = some ? 1.f / l : 0.f;
+        // a row that sees no key has zeros, one that sees scores of -infinity alone 0 / 0
+        const bool some = sees > 0, mine = tok < q.lq;
+        if (m == -INFINITY) l *= 0.f;         // next to nothing from exp2_by_products, or a NaN from before the row's last keys
+        const float inv = 1.f / l;
         const uint32_t head = head_of(x);
         __half *out = static_cast<__half *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(head) * a.head;
 #pragma unroll
@@ -439,7 +441,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
             }
           }
         }
-        if (a.lse && mine) a.lse[static_cast<unsigned long long>(head) * a.rows_q + q.q0 + tok] = some ? m * to2 * kLn2 + logf(l) : -INFINITY;
+        if (a.lse && mine) a.lse[static_cast<unsigned long long>(head) * a.rows_q + q.q0 + tok] = some ? (m == -INFINITY ? 0.f : m * to2 * kLn2) + logf(l) : -INFINITY;
       }
     }
   }
@@ -668,14 +670,15 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
           for (uint32_t c = 0; c < 4; ++c) {
             const uint32_t tok = from + t * kTile + c * 32u + lane;
             const unsigned long long at = stat + static_cast<unsigned long long>(g) * a.rows_q + tok;
-            lse[c] = tok < q.lq ? a.lse[at] : -INFINITY;
+            lse[c] = tok < q.lq ? a.lse[at] : 0.f;
             delta[c] = tok < q.lq ? a.delta[at] : 0.f;
           }
           // the numbers of two steps ago are done with when that step's ds is
           if (i >= kStats && !wait_all(smem_u32(&sh.ds_full[i & 1u]), ((i - kStats) >> 1) & 1u, abort_flag)) break;
 #pragma unroll
           for (uint32_t c = 0; c < 4; ++c) {
-            sh.stat[i % kStats][0][c * 32u + lane] = lse[c] == -INFINITY ? lse[c] : kPBits - lse[c] * kLog2e;
+            // (scores of -infinity alone have an lse of that too, and p is a NaN)
+            sh.stat[i % kStats][0][c * 32u + lane] = from + t * kTile + c * 32u + lane < q.lq ? kPBits - lse[c] * kLog2e : -INFINITY;
             sh.stat[i % kStats][1][c * 32u + lane] = -delta[c] * f;
           }
         }
@@ -760,14 +763,13 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
       float base = 0.f, minus_delta = 0.f;
       long long sees = q.lk;
       if constexpr (!kKeys) {
+        if (a.causal) sees = min(sees, max(0ll, static_cast<long long>(row) + 1 + shift));
         if (row < rows) {
-          const float lse = a.lse[stat + row];
-          base = lse == -INFINITY ? 0.f : -lse * kLog2e;   // (a query that sees nothing: every column below is masked)
+          base = sees > 0 ? -a.lse[stat + row] * kLog2e : 0.f;   // (a query that sees nothing: every column below is masked)
           const float delta = a.delta[stat + row];
           ds_scale = scale_of(a.gy_norm[stat + row], vm, fabsf(delta));
           minus_delta = -delta * ds_scale;
         }
-        if (a.causal) sees = min(sees, max(0ll, static_cast<long long>(row) + 1 + shift));
       }
       const float f = kKeys ? ds_scale * exp2f(-kPBits) : ds_scale;
       const f32x2 to22 = pair_of(to2, to2), f2 = pair_of(f, f), base2 = pair_of(base, base), minus_delta2 = pair_of(minus_delta, minus_delta);

@@ -286,7 +286,8 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
 #pragma unroll
     for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][threadIdx.x]);
 #pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) sum += s_m[w][threadIdx.x] == -INFINITY ? 0.f : exp2_of<T>(s_m[w][threadIdx.x] - top) * s_l[w][threadIdx.x];
+    for (uint32_t w = 0; w < kWarps; ++w)   // (a maximum of -infinity leaves out NaNs, so the sum counts all the same)
+      sum += (s_m[w][threadIdx.x] == -INFINITY ? 0.f : exp2_of<T>(s_m[w][threadIdx.x] - top)) * s_l[w][threadIdx.x];
     s_top[threadIdx.x] = top, s_sum[threadIdx.x] = sum;
   }
   __syncthreads();
@@ -322,11 +323,14 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
         sum += w * s_weight[r][threadIdx.x];
         s_weight[r][threadIdx.x] = w;
       }
-    const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+    // a row that sees no key has zeros, one that sees scores of -infinity alone 0 / 0
+    const uint32_t tok = (row0 + threadIdx.x) / a.group;
+    const bool sees = a.causal ? static_cast<long long>(tok) + shift >= 0 : q.lk > 0u;
+    const float inv = sees ? 1.f / sum : 0.f;
     for (uint32_t r = 0; r < splits; ++r) s_weight[r][threadIdx.x] *= inv;
     if (rank == 0 && a.lse && threadIdx.x < here) {
-      const uint32_t tok = (row0 + threadIdx.x) / a.group, h = hk * a.group + row0 + threadIdx.x - tok * a.group;
-      a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = top == -INFINITY ? -INFINITY : top * kLn2 + logf(sum);
+      const uint32_t h = hk * a.group + row0 + threadIdx.x - tok * a.group;
+      a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = sees ? (top == -INFINITY ? 0.f : top * kLn2) + logf(sum) : -INFINITY;
     }
   }
   __syncthreads();

@@ -543,3 +543,42 @@ def test_two_calls_at_once(ctx, mode):
     torch.cuda.synchronize()
     for p, w in zip(problems, want):
         assert all(torch.equal(a, b) for a, b in zip((p.y, p.lse, p.gq, p.gk, p.gv), w))
+
+
+# kernels of a forward pass: (head, queries, keys); a few queries, mma.sync with one block to a tile and with a cluster, tcgen05
+WAYS = [(64, 1, 100), (64, 3, 700), (40, 50, 90), (40, 50, 900), (33, 200, 900), (64, 200, 200), (128, 300, 520), (256, 1, 60), (256, 90, 90)]
+
+
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32", "tf32"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("head, lq, lk", WAYS)
+def test_rows_without_a_finite_score(ctx, mode, causal, head, lq, lk):
+    """A query with a NaN has y and lse of NaN; one whose scores are all -infinity has weights of 0 / 0, and a sum of zeros in lse; one with a score
+    of +infinity has infinity / infinity.  No other row is touched, and all three reach their gradients."""
+    p = Problem(mode, head, 4, 2, packed([lq]), packed([lk]), causal, seed=61)
+    p.k[:, :, 0] = abs(p.k[:, :, 0]) + 0.125      # so q = -inf here makes every score -inf
+    rows = sorted({0, lq // 2, lq - 1})
+    bad = {(r, h): (NAN, -math.inf, math.inf)[(i + h) % 3] for i, r in enumerate(rows) for h in (1, 2, 3)}
+    clean = p.q.clone()
+    for (r, h), v in bad.items():
+        p.q[r, h, 0] = v
+    p.forward(ctx)
+    hit = torch.zeros(lq, 4, dtype=torch.bool, device="cuda")
+    for (r, h), v in bad.items():
+        hit[r, h] = True
+        assert p.y[r, h].isnan().all(), (r, h, v)
+        lse = p.lse[h, r].item()
+        # (+infinity less itself is a NaN, and so is an infinity split into two parts of TF32)
+        assert math.isnan(lse) or lse == v and v < 0, (r, h, v, lse)
+        assert v != -math.inf or mode == "3xtf32" or lse == v, (r, h, v, lse)
+    y, lse = p.y.clone(), p.lse.clone()
+    assert not y[~hit].isnan().any() and lse.t()[~hit].isfinite().all()
+    p.backward(ctx)
+    assert p.gq[hit].isnan().all() and not p.gq[:, 0].isnan().any()
+    for (r, h), v in bad.items():
+        seen = r + lk - lq + 1 if causal else lk
+        assert p.gk[:seen, h // 2].isnan().all() and p.gv[:seen, h // 2].isnan().all()
+    p.q.copy_(clean)
+    p.forward(ctx)
+    assert torch.equal(p.y[~hit], y[~hit]) and torch.equal(p.lse.t()[~hit], lse.t()[~hit])
+    p.check()
