@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
       T *out = static_cast<T *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(h) * a.head + c;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < a.head) out[e] = round_to<T>(sees ? v[e] / sum : v[e]);
+        if (c + e < a.head) out[e] = round_to<T>(sees ? v[e] / sum : 0.f);
       if (a.lse && c == 0) a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = sees ? (top == -INFINITY ? 0.f : top * kLn2) + logf(sum) : -INFINITY;
     }
     cluster_sync_all();   // nobody leaves while another reads its part
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(128) attention_fw_kernel(AttnArgs a, uint32_t 
     // a row that sees no key has zeros, one that sees scores of -infinity alone 0 / 0; a maximum of -infinity also leaves out NaNs
     const bool sees = last[r] >= 0;
     store_row<T, kD>(static_cast<T *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(h) * a.head, acc, r, 0, a.head,
-                     sees ? 1.f / l[r] : 0.f, 0);
+                     1.f / l[r], 0, sees);
     if (a.lse && t == 0)
       a.lse[static_cast<unsigned long long>(h) * a.rows_q + q.q0 + tok] = sees ? (m[r] == -INFINITY ? 0.f : m[r] * kLn2) + logf(l[r]) : -INFINITY;
   }
@@ -370,15 +370,17 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
       }
       const float factor = which ? (kHalf ? 1.f / kPScale : 1.f) : undo;
       T *out;
+      bool some = true;
       if constexpr (kKeys) {
         out = which ? static_cast<T *>(a.gv) + (q.k0 + rw) * a.v_ld + hk_at : static_cast<T *>(a.gk) + (q.k0 + rw) * a.k_ld + hk_at;
       } else {
         const uint32_t tok = rw / a.group;
+        some = last_key(tok) >= 0;
         out = static_cast<T *>(a.gq) + (q.q0 + tok) * a.q_ld + hq_at + static_cast<unsigned long long>(rw - tok * a.group) * a.head;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < a.head) out[c + e] = round_to<T>(v[e] * factor + (a.accumulate ? static_cast<float>(out[c + e]) : 0.f));
+        if (c + e < a.head) out[c + e] = round_to<T>((some ? v[e] * factor : 0.f) + (a.accumulate ? static_cast<float>(out[c + e]) : 0.f));
     }
     cluster_sync_all();   // nobody leaves while another reads its part
     return;
@@ -392,7 +394,7 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
     } else {
       const uint32_t tok = row[r] / a.group;
       store_row<T, kCols>(static_cast<T *>(a.gq) + (q.q0 + tok) * a.q_ld + hq_at + static_cast<unsigned long long>(row[r] - tok * a.group) * a.head,
-                          acc2, r, col0, a.head, undo, a.accumulate);
+                          acc2, r, col0, a.head, undo, a.accumulate, row_last[r] >= 0);
     }
   }
 }

@@ -236,9 +236,10 @@ template <typename T> __device__ __forceinline__ T round_to(float v);
 template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
 
-// One row's columns of an accumulator: columns col0 + 8n + 2t, + 1.
+// One row's columns of an accumulator: columns col0 + 8n + 2t, + 1.  Zeros in their place where not `some`, whatever they are.
 template <typename T, int kCols>
-__device__ __forceinline__ void store_row(T *out, const float (&acc)[kCols / 8][4], int half, int col0, uint32_t head, float factor, int accumulate) {
+__device__ __forceinline__ void store_row(T *out, const float (&acc)[kCols / 8][4], int half, int col0, uint32_t head, float factor, int accumulate,
+                                          bool some = true) {
   const uint32_t t = threadIdx.x & 3u;
 #pragma unroll
   for (int n = 0; n < kCols / 8; ++n)
@@ -246,7 +247,7 @@ __device__ __forceinline__ void store_row(T *out, const float (&acc)[kCols / 8][
     for (int e = 0; e < 2; ++e) {
       const uint32_t c = col0 + n * 8 + 2 * t + e;
       if (c < head) {
-        float v = acc[n][half * 2 + e] * factor;
+        float v = some ? acc[n][half * 2 + e] * factor : 0.f;
         if (accumulate) v += static_cast<float>(out[c]);
         out[c] = round_to<T>(v);
       }

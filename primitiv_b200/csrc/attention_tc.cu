@@ -861,6 +861,7 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
         // of gq's columns each
         const bool is_v = kKeys && part < 2u;
         const float undo = is_v ? exp2f(-kPBits) : a.scale / ds_scale;
+        const bool some = steps > 0 && (kKeys || sees > 0);   // a query that sees no key has zeros, whatever it and the keys hold
         constexpr int kCols = kKeys ? kD / 2 : kD / 4;
         const uint32_t c0 = (kKeys ? part & 1u : part) * kCols;
         const uint32_t acc = tmem + lanes + (is_v ? kAcc1 : kAcc2) + c0;
@@ -879,7 +880,7 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
             if (row < rows && c0 + c + e < a.head) {
               float v[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) v[k] = steps > 0 ? __uint_as_float(y[e + k]) * undo : 0.f;
+              for (int k = 0; k < 8; ++k) v[k] = some ? __uint_as_float(y[e + k]) * undo : 0.f;
               uint4 *to16 = reinterpret_cast<uint4 *>(out + c0 + c + e);
               if (a.accumulate) {
                 const uint4 old = *to16;

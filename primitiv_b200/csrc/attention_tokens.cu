@@ -303,6 +303,8 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
   }
 
   // ---- the blocks' parts ----
+  // a query that sees no key has zeros, whatever the values that the others see hold
+  auto sees_any = [&](uint32_t tok) { return a.causal ? static_cast<long long>(tok) + shift >= 0 : q.lk > 0u; };
   if (splits > 1) cluster_sync_all();
   else __syncthreads();
   if (threadIdx.x < 16) {
@@ -323,10 +325,10 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
         sum += w * s_weight[r][threadIdx.x];
         s_weight[r][threadIdx.x] = w;
       }
-    // a row that sees no key has zeros, one that sees scores of -infinity alone 0 / 0
+    // (a row that sees scores of -infinity alone has 0 / 0)
     const uint32_t tok = (row0 + threadIdx.x) / a.group;
-    const bool sees = a.causal ? static_cast<long long>(tok) + shift >= 0 : q.lk > 0u;
-    const float inv = sees ? 1.f / sum : 0.f;
+    const bool sees = sees_any(tok);
+    const float inv = 1.f / sum;
     for (uint32_t r = 0; r < splits; ++r) s_weight[r][threadIdx.x] *= inv;
     if (rank == 0 && a.lse && threadIdx.x < here) {
       const uint32_t h = hk * a.group + row0 + threadIdx.x - tok * a.group;
@@ -346,9 +348,10 @@ __global__ void __launch_bounds__(kThreads) attention_tokens_kernel(AttnArgs a, 
     }
     const uint32_t tok = (row0 + at) / a.group, h = hk * a.group + row0 + at - tok * a.group;
     T *out = static_cast<T *>(a.y) + (q.q0 + tok) * a.y_ld + static_cast<unsigned long long>(h) * a.head + c;
+    const bool sees = sees_any(tok);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (c + e < a.head) out[e] = round_to<T>(v[e]);
+      if (c + e < a.head) out[e] = round_to<T>(sees ? v[e] : 0.f);
   }
   if (splits > 1) cluster_sync_all();   // nobody leaves while another reads its part
 }

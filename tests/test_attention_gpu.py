@@ -582,3 +582,34 @@ def test_rows_without_a_finite_score(ctx, mode, causal, head, lq, lk):
     p.forward(ctx)
     assert torch.equal(p.y[~hit], y[~hit]) and torch.equal(p.lse.t()[~hit], lse.t()[~hit])
     p.check()
+
+
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32", "tf32"])
+@pytest.mark.parametrize("bad", [NAN, math.inf])
+@pytest.mark.parametrize("head, lq, lk", [(64, 4, 2), (40, 60, 20), (40, 1200, 700), (256, 90, 30), (64, 300, 200), (128, 200, 90), (128, 400, 130)])
+def test_queries_that_see_no_key_are_zero_whatever_stands_in_the_keys(ctx, mode, bad, head, lq, lk):
+    """A causal sequence with more queries than keys: the first see nothing, whatever their q and gy, or any k and v of the sequence, hold."""
+    p = Problem(mode, head, 4, 2, packed([lq, lq]), packed([lk, lk]), True, seed=62)
+    none = torch.zeros(p.rows_q, dtype=torch.bool, device="cuda")
+    for first, n in p.q_at:
+        none[first:first + n - lk] = True
+    for t in (p.q, p.gy):
+        t[none] = bad
+    p.forward(ctx)
+    p.backward(ctx)
+    assert (p.y[none] == 0).all() and (p.lse[:, none] == -math.inf).all() and (p.gq[none] == 0).all()
+    clean = [t.clone() for t in (p.y, p.lse, p.gq, p.gk, p.gv)]
+    assert not any(t.isnan().any() for t in clean)
+    for t in (p.k, p.v):
+        t[::3] = bad
+    p.forward(ctx)
+    assert (p.y[none] == 0).all() and (p.lse[:, none] == -math.inf).all()
+    p.backward(ctx)
+    assert (p.gq[none] == 0).all()
+    # with zeros in those rows instead: the same bits everywhere
+    p = Problem(mode, head, 4, 2, packed([lq, lq]), packed([lk, lk]), True, seed=62)
+    for t in (p.q, p.gy):
+        t[none] = 0.0
+    p.forward(ctx)
+    p.backward(ctx)
+    assert all(torch.equal(a, b) for a, b in zip(clean, (p.y, p.lse, p.gq, p.gk, p.gv)))
