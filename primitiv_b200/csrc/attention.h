@@ -125,6 +125,15 @@ __device__ __forceinline__ float attn_exp2(float x) {
   return y;
 }
 
+// The scale of ds for halves: the power of two that takes the largest |ds| possible to at most 2^14.  |dp - delta| <= |gy| |v| + |delta|.
+__device__ __forceinline__ float attn_ds_scale(float gy_sq, float v_sq, float delta) {
+  const float bound = sqrtf(gy_sq) * sqrtf(v_sq) + delta;
+  if (!(bound > 1e-30f) || !(bound < 1e30f)) return 1.f;
+  return exp2f(fminf(fmaxf(13.f - ceilf(log2f(bound)), -100.f), 100.f));
+}
+// The larger one, without x if that is an infinity or a NaN: what holds one has such gradients whatever the scale, and the others keep theirs.
+__device__ __forceinline__ float attn_finite_max(float top, float x) { return x < INFINITY ? fmaxf(top, x) : top; }
+
 #endif  // __CUDACC__
 
 // The tiles of all sequences together, a bound, and how they are numbered.  Through all sequences there are few beyond those that exist, but

@@ -16,7 +16,7 @@
 // fp32 storage: a product is three TF32 passes on x = hi + lo split in registers (one in B200_MODE_TF32).  The tensor core
 // truncates as it adds into its accumulator, so no sum runs longer than one tile there: each tile's product starts from zero and
 // is added in fp32 instructions.  Halves: p and ds are rounded to half for the second product, ds after a scale by a power of
-// two (see scale_of), without which the ds of a long row, p / row length times a small gy, would lie below the
+// two (see attn_ds_scale), without which the ds of a long row, p / row length times a small gy, would lie below the
 // smallest half.
 #include <algorithm>
 #include "attention_mma.cuh"
@@ -183,13 +183,6 @@ template <typename T, int kD> constexpr int kBwThreads = kD == 256 ? 256 : 128; 
 template <typename T, int kD> constexpr int kBwStages = sizeof(T) == 4 ? 1 : 2;
 template <typename T, int kD> constexpr int kBwBlocks = sizeof(T) == 4 && kD == 64 ? 3 : 1;
 
-// The power of two that takes the largest |ds| possible to at most 2^14.  |dp - delta| <= |gy| |v| + |delta|.
-__device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) {
-  const float bound = sqrtf(gy_sq) * sqrtf(v_sq) + delta;
-  if (!(bound > 1e-30f) || !(bound < 1e30f)) return 1.f;
-  return exp2f(fminf(fmaxf(13.f - ceilf(log2f(bound)), -100.f), 100.f));
-}
-
 // kKeys: the keys rest, the queries of all heads of the group pass by (gk, gv).  Else the queries rest (gq).
 template <typename T, int kD, int kPass, bool kKeys>
 __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nth, uint32_t tiles, uint32_t splits, int wide) {
@@ -200,7 +193,7 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
   constexpr float kLseUnit = kHalf ? kLog2e : 1.f;
   extern __shared__ __align__(16) unsigned char s_raw[];
   __shared__ uint32_t s_at[2];
-  __shared__ float s_lse[2][BN], s_delta[2][BN], s_max[3][8];
+  __shared__ float s_lse[2][BN], s_delta[2][BN], s_max[3][8], s_undo[kRows];
   __shared__ int s_last[2][BN];   // the last key that a query sees
   T *x1 = reinterpret_cast<T *>(s_raw), *x2 = x1 + kRows * P, *y1 = x2 + kRows * P, *y2 = y1 + kStages * BN * P;
   uint32_t seq, tile;
@@ -261,19 +254,23 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
   if (steps) load_step(0, 0);
   else copies_commit();
 
-  float ds_scale = 1.f;
-  if constexpr (kHalf) {   // over all that this block sees: the scale must not change on the way
-    const uint32_t q_from = kKeys ? from : row0, q_to = kKeys ? qrows : min(row0 + kRows, rows);
+  // Scale of ds: with the keys at rest one for all that this block sees, since it must not change on the way; with the queries at rest one per
+  // query, so that none loses bits to another with a larger gradient.
+  float ds_scale[2] = {1.f, 1.f};
+  float vm = 0.f;
+  if constexpr (kHalf) {
     const uint32_t k_from = kKeys ? row0 : 0u, k_to = kKeys ? min(row0 + kRows, rows) : to;
-    float gm = 0.f, dm = 0.f, vm = 0.f;
-    for (uint32_t r = q_from + threadIdx.x; r < q_to; r += kThreads) {
-      const uint32_t tok = r / a.group;
-      const unsigned long long i = stat + static_cast<unsigned long long>(r - tok * a.group) * a.rows_q + tok;
-      gm = fmaxf(gm, a.gy_norm[i]);
-      dm = fmaxf(dm, fabsf(a.delta[i]));
+    float gm = 0.f, dm = 0.f;
+    if constexpr (kKeys) {
+      for (uint32_t r = from + threadIdx.x; r < qrows; r += kThreads) {
+        const uint32_t tok = r / a.group;
+        const unsigned long long i = stat + static_cast<unsigned long long>(r - tok * a.group) * a.rows_q + tok;
+        gm = attn_finite_max(gm, a.gy_norm[i]);
+        dm = attn_finite_max(dm, fabsf(a.delta[i]));
+      }
     }
     for (uint32_t r = k_from + threadIdx.x; r < k_to; r += kThreads)
-      vm = fmaxf(vm, a.v_norm[static_cast<unsigned long long>(hk) * a.rows_k + q.k0 + r]);
+      vm = attn_finite_max(vm, a.v_norm[static_cast<unsigned long long>(hk) * a.rows_k + q.k0 + r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
@@ -284,7 +281,7 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < kThreads / 32; ++w) gm = fmaxf(gm, s_max[0][w]), dm = fmaxf(dm, s_max[1][w]), vm = fmaxf(vm, s_max[2][w]);
-    ds_scale = scale_of(gm, vm, dm);
+    if constexpr (kKeys) ds_scale[0] = ds_scale[1] = attn_ds_scale(gm, vm, dm);
   }
 
   uint32_t row[2];
@@ -299,6 +296,7 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
       const unsigned long long at = stat + static_cast<unsigned long long>(row[r] - tok * a.group) * a.rows_q + tok;
       row_lse[r] = a.lse[at] * kLseUnit;
       row_delta[r] = a.delta[at];
+      if constexpr (kHalf) ds_scale[r] = attn_ds_scale(a.gy_norm[at], vm, fabsf(row_delta[r]));
     }
   }
   float acc1[kKeys ? kCols / 8 : 1][4], acc2[kCols / 8][4];
@@ -336,27 +334,29 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
           const bool seen = kKeys ? row_last[r] <= col_last : key <= row_last[r];
           const float lse = kKeys ? col_lse : row_lse[r];
           const float x = !seen ? 0.f : kHalf ? exp2_of<T>(fmaf(p[n][i], to2, -lse)) : exp2_of<T>(fmaf(p[n][i], a.scale, -lse) * kLog2e);
-          ds[n][i] = seen ? x * (ds[n][i] - (kKeys ? col_delta : row_delta[r])) * ds_scale : 0.f;
+          ds[n][i] = seen ? x * (ds[n][i] - (kKeys ? col_delta : row_delta[r])) * ds_scale[r] : 0.f;
           p[n][i] = kHalf ? x * kPScale : x;
         }
       }
     if constexpr (kKeys) product_py<kD, kCols, NT, kPass>(acc1, p, y2 + at * BN * P, col0, 1.f, 1.f);
     product_py<kD, kCols, NT, kPass>(acc2, ds, y1 + at * BN * P, col0, 1.f, 1.f);
   }
-  const float undo = a.scale / ds_scale;
+  const float undo[2] = {a.scale / ds_scale[0], a.scale / ds_scale[1]};
   if (splits > 1) {
     // the blocks' sums: each lays down its own, and adds the rows that fall to it, in rank order
     float *part = reinterpret_cast<float *>(s_raw);
     copies_wait<0>();
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < 2; ++r) {
+      if (t == 0) s_undo[wrow + g + r * 8] = undo[r];
 #pragma unroll
       for (int n = 0; n < kCols / 8; ++n) {
         float *at = part + (wrow + g + r * 8) * kD + col0 + n * 8 + 2 * t;
         *reinterpret_cast<float2 *>(at) = make_float2(acc2[n][2 * r], acc2[n][2 * r + 1]);
         if constexpr (kKeys) *reinterpret_cast<float2 *>(at + kRows * kD) = make_float2(acc1[n][2 * r], acc1[n][2 * r + 1]);
       }
+    }
     cluster_sync_all();
     const uint32_t mine = kRows / splits, at0 = rank * mine;
     for (uint32_t i = threadIdx.x; i < (kKeys ? 2u : 1u) * mine * (kD / 4); i += kThreads) {
@@ -368,7 +368,7 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
         const float4 o = ld_cluster4(map_to_cta(smem_at(part + (which * kRows + at) * kD + c), s));
         v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
       }
-      const float factor = which ? (kHalf ? 1.f / kPScale : 1.f) : undo;
+      const float factor = which ? (kHalf ? 1.f / kPScale : 1.f) : s_undo[at];
       T *out;
       bool some = true;
       if constexpr (kKeys) {
@@ -390,11 +390,11 @@ __device__ __forceinline__ void attention_bw_side(const AttnArgs &a, uint32_t nt
     if (row[r] >= rows) continue;
     if constexpr (kKeys) {
       store_row<T, kCols>(static_cast<T *>(a.gv) + (q.k0 + row[r]) * a.v_ld + hk_at, acc1, r, col0, a.head, kHalf ? 1.f / kPScale : 1.f, a.accumulate);
-      store_row<T, kCols>(static_cast<T *>(a.gk) + (q.k0 + row[r]) * a.k_ld + hk_at, acc2, r, col0, a.head, undo, a.accumulate);
+      store_row<T, kCols>(static_cast<T *>(a.gk) + (q.k0 + row[r]) * a.k_ld + hk_at, acc2, r, col0, a.head, undo[r], a.accumulate);
     } else {
       const uint32_t tok = row[r] / a.group;
       store_row<T, kCols>(static_cast<T *>(a.gq) + (q.q0 + tok) * a.q_ld + hq_at + static_cast<unsigned long long>(row[r] - tok * a.group) * a.head,
-                          acc2, r, col0, a.head, undo, a.accumulate, row_last[r] >= 0);
+                          acc2, r, col0, a.head, undo[r], a.accumulate, row_last[r] >= 0);
     }
   }
 }

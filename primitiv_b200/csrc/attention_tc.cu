@@ -504,13 +504,6 @@ struct BwShared {
 };
 static_assert(sizeof(BwShared) <= kBwHead, "no room");
 
-// The power of two that takes the largest |ds| possible to at most 2^14.  |dp - delta| <= |gy| |v| + |delta|.
-__device__ __forceinline__ float scale_of(float gy_sq, float v_sq, float delta) {
-  const float bound = sqrtf(gy_sq) * sqrtf(v_sq) + delta;
-  if (!(bound > 1e-30f) || !(bound < 1e30f)) return 1.f;
-  return exp2f(fminf(fmaxf(13.f - ceilf(log2f(bound)), -100.f), 100.f));
-}
-
 // A position in a ring.
 template <uint32_t kSlots>
 struct Slot {
@@ -589,14 +582,14 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
 #pragma unroll 4
           for (uint32_t t = from + threadIdx.x; t < q.lq; t += kBwThreads) {
             const unsigned long long i = stat + static_cast<unsigned long long>(g) * a.rows_q + t;
-            gm = fmaxf(gm, a.gy_norm[i]);
-            dm = fmaxf(dm, fabsf(a.delta[i]));
+            gm = attn_finite_max(gm, a.gy_norm[i]);
+            dm = attn_finite_max(dm, fabsf(a.delta[i]));
           }
       }
       const uint32_t k_from = kKeys ? row0 : 0u, k_to = kKeys ? min(row0 + kTile, rows) : to;
 #pragma unroll 4
       for (uint32_t t = k_from + threadIdx.x; t < k_to; t += kBwThreads)
-        vm = fmaxf(vm, a.v_norm[static_cast<unsigned long long>(kv_head) * a.rows_k + q.k0 + t]);
+        vm = attn_finite_max(vm, a.v_norm[static_cast<unsigned long long>(kv_head) * a.rows_k + q.k0 + t]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
@@ -607,7 +600,7 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
       __syncthreads();
 #pragma unroll
       for (uint32_t w = 0; w < kBwThreads / 32; ++w) gm = fmaxf(gm, sh.top[0][w]), dm = fmaxf(dm, sh.top[1][w]), vm = fmaxf(vm, sh.top[2][w]);
-      ds_scale = scale_of(gm, vm, dm);
+      ds_scale = attn_ds_scale(gm, vm, dm);
     }
 
     if (warp == 1) {
@@ -767,7 +760,7 @@ __device__ __forceinline__ void attention_bw_side(const BwParams &p, uint8_t *sm
         if (row < rows) {
           base = sees > 0 ? -a.lse[stat + row] * kLog2e : 0.f;   // (a query that sees nothing: every column below is masked)
           const float delta = a.delta[stat + row];
-          ds_scale = scale_of(a.gy_norm[stat + row], vm, fabsf(delta));
+          ds_scale = attn_ds_scale(a.gy_norm[stat + row], vm, fabsf(delta));
           minus_delta = -delta * ds_scale;
         }
       }

@@ -613,3 +613,23 @@ def test_queries_that_see_no_key_are_zero_whatever_stands_in_the_keys(ctx, mode,
     p.forward(ctx)
     p.backward(ctx)
     assert all(torch.equal(a, b) for a, b in zip(clean, (p.y, p.lse, p.gq, p.gk, p.gv)))
+
+
+@pytest.mark.parametrize("head", [128, 40, 33, 256])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("big", [3e4, math.inf])
+def test_a_query_beside_one_with_a_huge_gradient(ctx, head, causal, big):
+    """Gradients of queries do not mix: rows whose gy is 2^-14 keep their bits in a tile with rows of 3e4, or of infinities."""
+    at = packed([700])
+    p = Problem("fp16", head, 2, 1, at, at, causal, seed=63, gy_size=2.0 ** -14)
+    loud = torch.zeros(700, dtype=torch.bool, device="cuda")
+    loud[[3, 64, 130, 131, 400, 699]] = True
+    p.gy[loud] = math.copysign(1.0, big) * big
+    p.forward(ctx)
+    p.backward(ctx)
+    for h in range(2):
+        gy = p.gy[:, h].double()
+        gy[loud] = 0.0          # what the others' gradients may lose is counted from their own gy
+        val, tol = attention(p.q[:, h].double(), p.k[:, 0].double(), p.v[:, 0].double(), p.scale, causal, gy, "fp16")
+        off = abs(p.gq[:, h].double() - val["gq"]) - tol["gq"]
+        assert not (off[~loud] > 0).any() and not p.gq[~loud, h].isnan().any(), off[~loud].max().item()
