@@ -101,6 +101,8 @@ B200_API int b200_norm_rotary_bw(b200_ctx *ctx, int mode, const void *x, const v
  * the same call.  The arrays are on the DEVICE and are read by the kernels: a captured graph follows
  * them.  max_q / max_k say how long a sequence can be (0: not known); longer ones are cut.  They
  * choose the kernel: max_q = 1 is a step of generation.
+ * Rows times heads, on either side, may be 2^31 - 2^16 at most, and heads_q * head less than 2^31
+ * (B200_ERR_TOO_LARGE); offsets in elements may pass 32 bits.
  *
  * Rows of y and lse that belong to no sequence are left as they were.  Gradients of such rows are zero:
  * stored with accumulate = 0, left alone with 1. */

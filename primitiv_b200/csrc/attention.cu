@@ -109,9 +109,10 @@ int check_plan(const b200_attention *p, AttnArgs *a) {
   if (!p || p->head == 0 || p->heads_q == 0 || p->heads_k == 0 || p->heads_q % p->heads_k != 0) return B200_ERR_INVALID_ARG;
   if (p->head > kAttnMaxHead) return B200_ERR_TOO_LARGE;
   if (!std::isfinite(p->scale)) return B200_ERR_INVALID_ARG;
-  // tiles are numbered in 32 bits
-  if (static_cast<u64>(p->rows_q) * p->heads_q > 0x7fffffffu || static_cast<u64>(p->rows_k) * p->heads_k > 0x7fffffffu || p->seqs > 0x3fffffffu ||
-      p->heads_k > 65535u)
+  // Tiles, the rows of one that ends behind the last row, and the elements of a token are numbered in 32 bits.
+  constexpr u64 kMostRows = 0x7fff0000u;
+  if (static_cast<u64>(p->rows_q) * p->heads_q > kMostRows || static_cast<u64>(p->rows_k) * p->heads_k > kMostRows || p->seqs > 0x3fffffffu ||
+      p->heads_k > 65535u || static_cast<u64>(p->heads_q) * p->head > 0x7fffffffu)
     return B200_ERR_TOO_LARGE;
   *a = AttnArgs{};
   a->head = p->head, a->heads_q = p->heads_q, a->heads_k = p->heads_k, a->group = p->heads_q / p->heads_k;

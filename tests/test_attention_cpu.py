@@ -105,6 +105,20 @@ def test_refused_plans(code, more):
     assert e.value.code == code
 
 
+@pytest.mark.parametrize("more", [dict(rows_k=(1 << 31) - 1, heads_k=1, head=1), dict(rows_q=(1 << 31) - 1, heads_q=1, heads_k=1, head=1),
+                                  dict(rows_q=1, heads_q=1 << 24, heads_k=1, head=256)])
+def test_sizes_whose_indexes_would_wrap_are_refused(more):
+    """A tile that ends behind the last row, and the elements of a token, are counted in 32 bits."""
+    with pytest.raises(pb.B200Error) as e:
+        plan(**more).bw_scratch_floats()
+    assert e.value.code == 1006
+
+
+def test_the_largest_sizes_are_taken():
+    assert plan(rows_k=(1 << 31) - (1 << 16), heads_k=1, head=1).bw_scratch_floats() == 2 * 100 * 8 + (1 << 31) - (1 << 16)
+    assert plan(rows_q=1, heads_q=1 << 22, heads_k=1, head=256).bw_scratch_floats() == (2 << 22) + 70
+
+
 def test_entry_points_refuse_a_null_context_and_plan():
     lib, n = pb.lib(), ctypes.c_uint64()
     p = ctypes.addressof(plan())
