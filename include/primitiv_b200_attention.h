@@ -48,8 +48,9 @@ B200_API int b200_rotary_frequencies(uint32_t rot, double base, int scaling, dou
                                      double *freqs_host, double *amplitude_host);
 
 /* y = turned x; gx (+)= gy turned back, the transposed map.  head <= 256, rot even and <= head.
- * `freqs`: rot/2 doubles on the device (angles are formed and reduced in 64 bits, so positions of any
- * size keep the precision of the values).  `positions`: one per token, or NULL for 0, 1, 2, ...
+ * `freqs`: rot/2 doubles on the device.  `positions`: one per token, or NULL for 0, 1, 2, ...  Angles
+ * position * freqs[pair] are formed and reduced in 64 bits, far positions with what the products round off, and
+ * rounded to 32 bits then: at any position they are right to 2^-26 of a turn.
  * y may be x, and gx may be gy, with the same ld and without accumulate. */
 B200_API int b200_rotary_fw(b200_ctx *ctx, int mode, const void *x, void *y, uint32_t head, uint32_t heads,
                             uint32_t tokens, uint64_t x_ld, uint64_t y_ld, uint32_t rot, int layout,

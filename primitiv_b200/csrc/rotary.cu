@@ -14,8 +14,8 @@
 // group stays with one token and goes over its heads, with the token's cosines and the gain in registers; arithmetic is on pairs of floats.
 // (A group that took any row, and read cosines and gain for it, spent two to three times the instructions: 71 us forward, 91 us with norms,
 // 266 us for their gradient, where this takes 62, 84 and 116; 16384 tokens of 40 heads of 128 halves.)
-// An angle is formed in turns and reduced in 64 bits, so position 1000000 has the same error (2^-26 of a turn) as position
-// 0; its sine and cosine are 32-bit.
+// An angle is formed in turns, with what its products round off, and reduced in 64 bits, so the last position, 2^32 - 1, has the same
+// error (2^-26 of a turn) as position 1; its sine and cosine are 32-bit.
 //
 // With norms a block takes the heads of one gain only.  Gradients of gains are sums over every token and head: a thread keeps its
 // elements' sums in registers over all that its block takes, a block writes one partial row and a second kernel adds the
@@ -277,9 +277,13 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
     for (uint32_t i = threadIdx.x; i < nt * pairs; i += kThreads) {
       const uint32_t t = i / pairs, p = i - t * pairs;
       const double pos = a.positions ? static_cast<double>(a.positions[t0 + t]) : static_cast<double>(t0 + t);
-      const double turns = pos * (a.freqs[p] * 0.15915494309189533577);   // 1 / (2 pi)
+      constexpr double kTurn = 0.15915494309189533577, kTurnRest = -9.839338337591243477e-18;   // 1 / (2 pi) in two doubles
+      const double freq = a.freqs[p], step = freq * kTurn, turns = pos * step;
+      double part = turns - rint(turns);
+      // far out a product's half bit is up to 2^-24 of a turn: what the two have rounded off (before 2^20 turns it is less than 2^-31)
+      if (fabs(turns) > 1048576.0) part += ::fma(pos, step, -turns) + pos * (::fma(freq, kTurn, -step) + freq * kTurnRest);
       float sn, cs;
-      sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+      sincospif(2.f * static_cast<float>(part), &sn, &cs);
       s_tab[t * tab_size + (p % V) * pitch + p / V] = make_float2(a.amplitude * cs, a.amplitude * (kBack ? -sn : sn));
     }
     if constexpr (kStaged) asm volatile("cp.async.wait_group 0;" ::: "memory");

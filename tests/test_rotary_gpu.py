@@ -310,3 +310,29 @@ def test_an_epsilon_of_zero(ctx, mode, t, hq, hk, d, rot):
                        scratch.data_ptr(), d, hq, hk, t, 0, 0, 0, rot, PAIRS, f.data_ptr(), eps=0.0, accumulate_x=False, accumulate_gain=False)
     for value, exact, bound in ((got, gx, e_gx), (gg[0], ggq, e_q), (gg[1], ggk, e_k)):
         assert (abs(value.double() - exact) <= bound + store * (abs(exact) + bound) + tiny).all()
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("layout", [PAIRS, HALVES])
+def test_angles_are_as_good_far_out_as_near_zero(ctx, layout, back):
+    """fp32 at positions up to the last one, against angles reduced in exact arithmetic: the bound that holds near position 0."""
+    from fractions import Fraction
+    two_pi = 2 * Fraction(314159265358979323846264338327950288419716939937510, 10 ** 50)
+    pos, rot = [0, 5, 16777217, 999999937, (1 << 32) - 1] + [(1 << 31) + i * 7158279 for i in range(300)], 32
+    freqs = pb.rotary_frequencies(rot)[0]
+    angles = torch.tensor([[float(p * Fraction(f) % two_pi) for f in freqs] for p in pos], device="cuda", dtype=torch.float64)
+    x = torch.randn(len(pos), 3, 40, device="cuda", generator=torch.Generator(device="cuda").manual_seed(81))
+    at = torch.tensor([p - (1 << 32) if p >> 31 else p for p in pos], device="cuda", dtype=torch.int32)
+    f, y = torch.tensor(freqs, device="cuda", dtype=torch.float64), torch.empty_like(x)
+    if back:
+        ctx.rotary_bw(0, x.data_ptr(), y.data_ptr(), 40, 3, len(pos), 0, 0, rot, layout, f.data_ptr(), positions=at.data_ptr(), accumulate=False)
+    else:
+        ctx.rotary_fw(0, x.data_ptr(), y.data_ptr(), 40, 3, len(pos), 0, 0, rot, layout, f.data_ptr(), positions=at.data_ptr())
+    want = rotary(x.double(), angles, 1.0, rot, layout, back=back)
+    # The angle in turns is rounded to 32 bits once, 2^-26 of a turn: 2 pi 2^-26 = 1.6 F32 of the pair's size; sine and cosine are right to
+    # 2 units each (2 sqrt(2) F32 of the pair); a product and the sum round once (2 F32).
+    pair = torch.view_as_complex(x[..., :rot].double().reshape(len(pos), 3, rot // 2, 2)).abs() if layout == PAIRS \
+        else torch.hypot(x[..., :rot // 2].double(), x[..., rot // 2:rot].double())
+    size = pair.repeat_interleave(2, -1) if layout == PAIRS else torch.cat((pair, pair), -1)
+    assert (abs(y.double() - want)[..., :rot] <= size * 7 * F32).all()
+    assert torch.equal(y[..., rot:], x[..., rot:])
