@@ -167,15 +167,6 @@ __device__ __forceinline__ void load_raw(Raw<T, V> &raw, const T *p, uint32_t c0
   if (c0 < head) raw.first = *reinterpret_cast<const Pack<T, V> *>(p + c0);
   if (c1 < head) raw.second = *reinterpret_cast<const Pack<T, V> *>(p + c1);
 }
-// The same element by element, from any address.
-template <typename T, int V>
-__device__ __forceinline__ void load_raw_any(Raw<T, V> &raw, const T *p, uint32_t c0, uint32_t c1, uint32_t head) {
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (c0 < head) raw.first.v[j] = p[c0 + j];
-    if (c1 < head) raw.second.v[j] = p[c1 + j];
-  }
-}
 // What there is none of counts as zero.
 template <typename T, int V, int kLayout>
 __device__ __forceinline__ Unit<V> unit_of(const Raw<T, V> &raw, bool has0, bool has1) {
@@ -239,7 +230,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   constexpr bool kStaged = kSums && kUnits == 1 && V * sizeof(T) >= 8;
   constexpr uint32_t kStages = 2;   // (three or four: the same time)
   extern __shared__ float2 s_tab[];                                  // [token][V][pitch]
-  __shared__ float s_sums[kSums ? kWarps * kMaxHead : 1];
+  __shared__ __align__(16) float s_sums[kSums ? kWarps * kMaxHead : (kNorm ? kMaxHead : 1)];   // the gain, and in the end the warps' sums
   __shared__ __align__(16) Pack<T, V> s_slots[kStaged ? kStages * 4 : 1][kThreads];
 
   const bool second = blockIdx.x >= a.blocks_q;
@@ -260,14 +251,13 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   }
   Unit<V> gain[kNorm ? kUnits : 1], sums[kSums ? kUnits : 1];
   if constexpr (kNorm) {
+    // Element by element, so that gains may begin anywhere in a buffer of parameters; every thread takes its own from here.
+    static_assert(kMaxHead <= kThreads, "one element a thread");
+    if (threadIdx.x < a.head) s_sums[threadIdx.x] = to_float(static_cast<const T *>(second ? a.gain_k : a.gain_q)[threadIdx.x]);
+  }
+  if constexpr (kSums) {
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      Raw<T, V> raw;
-      // (once in a block, so it need not be in vectors, and gains may begin at any element of a buffer of parameters)
-      load_raw_any(raw, static_cast<const T *>(second ? a.gain_k : a.gain_q), c0[k], c1[k], a.head);
-      gain[k] = unit_of<T, V, kLayout>(raw, c0[k] < a.head, c1[k] < a.head);
-      if constexpr (kSums) sums[k].a = sums[k].b = all_of<V>(0.f);
-    }
+    for (int k = 0; k < kUnits; ++k) sums[k].a = sums[k].b = all_of<V>(0.f);
   }
   const float per_head = 1.f / static_cast<float>(a.head);
 
@@ -325,6 +315,16 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
       fetch(0);
     }
     __syncthreads();
+    if constexpr (kNorm) {
+      if (tile == block) {
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+          Raw<float, V> raw;
+          load_raw(raw, s_sums, c0[k], c1[k], a.head);
+          gain[k] = unit_of<float, V, kLayout>(raw, c0[k] < a.head, c1[k] < a.head);
+        }
+      }
+    }
     Unit<V> cs[kUnits];   // a: cosine, b: sine
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
         w[k] = unit_of<T, V, kLayout>(raw[k], here && c0[k] < a.head, here && c1[k] < a.head);
         if constexpr (kSums) gw[k] = unit_of<T, V, kLayout>(raw_g[k], here && c0[k] < a.head, here && c1[k] < a.head);
       }
+      float ss = 0.f, dot = 0.f;
       if constexpr (kNorm) {
         Lane<V> sq = all_of<V>(0.f), dots = all_of<V>(0.f);
 #pragma unroll
@@ -370,24 +371,27 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
             dots = fma(gw[k].b * gain[k].b, w[k].b, fma(gw[k].a * gain[k].a, w[k].a, dots));
           }
         }
-        float ss = sum_of(sq), dot = kBack ? sum_of(dots) : 0.f;
+        ss = sum_of(sq);
+        if constexpr (kBack) dot = sum_of(dots);
         group_sums(ss, dot, a.lanes_log2);
-        const float rs = here ? rsqrtf(ss * per_head + a.eps) : 0.f;   // (without a row, eps = 0 would make it infinite, and 0 * rs a NaN in the sums)
-        const Lane<V> rs_all = all_of<V>(rs);
-        if constexpr (!kBack) {
+      }
+      if (here) {   // (without a row, an eps of 0 would make NaNs, which the sums keep)
+        if constexpr (kNorm) {
+          const float rs = rsqrtf(ss * per_head + a.eps);
+          const Lane<V> rs_all = all_of<V>(rs);
+          if constexpr (!kBack) {
 #pragma unroll
-          for (int k = 0; k < kUnits; ++k) w[k].a = w[k].a * (rs_all * gain[k].a), w[k].b = w[k].b * (rs_all * gain[k].b);
-        } else {
-          const Lane<V> minus_dot = all_of<V>(-per_head * rs * dot);
+            for (int k = 0; k < kUnits; ++k) w[k].a = w[k].a * (rs_all * gain[k].a), w[k].b = w[k].b * (rs_all * gain[k].b);
+          } else {
+            const Lane<V> minus_dot = all_of<V>(-per_head * rs * dot);
 #pragma unroll
-          for (int k = 0; k < kUnits; ++k) {
-            w[k].a = w[k].a * rs_all, w[k].b = w[k].b * rs_all;          // n; zero where there is no row
-            sums[k].a = fma(gw[k].a, w[k].a, sums[k].a), sums[k].b = fma(gw[k].b, w[k].b, sums[k].b);
-            w[k].a = rs_all * fma(w[k].a, minus_dot, gw[k].a * gain[k].a), w[k].b = rs_all * fma(w[k].b, minus_dot, gw[k].b * gain[k].b);
+            for (int k = 0; k < kUnits; ++k) {
+              w[k].a = w[k].a * rs_all, w[k].b = w[k].b * rs_all;          // n
+              sums[k].a = fma(gw[k].a, w[k].a, sums[k].a), sums[k].b = fma(gw[k].b, w[k].b, sums[k].b);
+              w[k].a = rs_all * fma(w[k].a, minus_dot, gw[k].a * gain[k].a), w[k].b = rs_all * fma(w[k].b, minus_dot, gw[k].b * gain[k].b);
+            }
           }
         }
-      }
-      if (here) {
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
           if constexpr (!kSums) turn(w[k], k);
@@ -409,6 +413,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
 
   if constexpr (kSums) {
     if (!a.partial) return;
+    __syncthreads();   // the gain's last readers are done
     const uint32_t warp = threadIdx.x >> 5;
 #pragma unroll
     for (int k = 0; k < kUnits; ++k)
