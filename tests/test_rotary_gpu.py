@@ -336,3 +336,24 @@ def test_angles_are_as_good_far_out_as_near_zero(ctx, layout, back):
     size = pair.repeat_interleave(2, -1) if layout == PAIRS else torch.cat((pair, pair), -1)
     assert (abs(y.double() - want)[..., :rot] <= size * 7 * F32).all()
     assert torch.equal(y[..., rot:], x[..., rot:])
+
+
+@pytest.mark.parametrize("mode", ["fp16", "3xtf32"])
+@pytest.mark.parametrize("t, hq, hk, d, rot, layout", [(20011, 2, 1, 32, 32, HALVES), (9001, 1, 1, 33, 6, PAIRS), (40003, 1, 2, 64, 16, PAIRS)])
+def test_norm_gradients_over_many_tiles(ctx, mode, t, hq, hk, d, rot, layout):
+    """More tokens than the blocks take at a time: a block goes from tile to tile, each with angles of its own."""
+    code, dtype = MODES[mode][:2]
+    store, tiny = store_rounding(dtype)
+    (x, _), (gy, _) = (inputs((t, hq + hk, d), dtype, seed) for seed in (91, 92))
+    gain_q, gain_k = (1 + 0.3 * torch.randn(2, d, device="cuda")).to(dtype)
+    positions = torch.randint(0, 1 << 20, (t,), device="cuda", dtype=torch.int32)
+    f = torch.tensor(pb.rotary_frequencies(rot)[0], device="cuda", dtype=torch.float64)
+    gx, ggq, ggk, e_gx, e_q, e_k = norm_reference(x, gain_q, gain_k, hq, positions.double()[:, None] * f, 1.0, rot, layout, 1e-5, gy)
+    got, gg, scratch = torch.empty_like(x), torch.empty(2, d, device="cuda", dtype=dtype), torch.empty(pb.NORM_ROTARY_SCRATCH, device="cuda")
+    ctx.norm_rotary_bw(code, x.data_ptr(), gain_q.data_ptr(), gain_k.data_ptr(), gy.data_ptr(), got.data_ptr(), gg[0].data_ptr(), gg[1].data_ptr(),
+                       scratch.data_ptr(), d, hq, hk, t, 0, 0, 0, rot, layout, f.data_ptr(), 1.0, positions.data_ptr(), 1e-5, accumulate_x=False,
+                       accumulate_gain=False)
+    # (the sums' bound takes 64 roundings one on another: at most 32 rows of heads in a thread here, 5 between lanes, 8 warps, 14 blocks, 32 lanes of those;
+    # each is of a part of the sum, and the bound's terms are all of it, with a factor 2)
+    for value, exact, bound in ((got, gx, e_gx), (gg[0], ggq, e_q), (gg[1], ggk, e_k)):
+        assert (abs(value.double() - exact) <= bound + store * (abs(exact) + bound) + tiny).all()
