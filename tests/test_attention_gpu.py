@@ -633,3 +633,14 @@ def test_a_query_beside_one_with_a_huge_gradient(ctx, head, causal, big):
         val, tol = attention(p.q[:, h].double(), p.k[:, 0].double(), p.v[:, 0].double(), p.scale, causal, gy, "fp16")
         off = abs(p.gq[:, h].double() - val["gq"]) - tol["gq"]
         assert not (off[~loud] > 0).any() and not p.gq[~loud, h].isnan().any(), off[~loud].max().item()
+
+
+def test_fp32_gradients_leave_the_scratch_of_halves_alone(ctx):
+    """Squares' sums are for the scales of halves: other modes neither read all of v for them nor store any."""
+    at = packed([130, 40], gap=2)
+    p = Problem("3xtf32", 64, 4, 2, at, at, True, seed=65, gap=3)
+    p.forward(ctx)
+    p.backward(ctx)
+    p.check(gradients=True)
+    used = p.rows_q * p.hq
+    assert p.scratch[used:].isnan().all() and not p.scratch[:used].view(p.hq, p.rows_q)[:, :130].isnan().any()
