@@ -24,6 +24,7 @@
 #include <cmath>
 
 #include "../../include/primitiv_b200_attention.h"
+#include "f32x2.cuh"
 #include "ops_common.cuh"
 
 namespace b200 {
@@ -80,25 +81,6 @@ __device__ __forceinline__ void unit_at(uint32_t u, uint32_t rot, uint32_t &c0, 
   c1 = c0 + V;
 }
 
-// Pairs of floats.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair_of(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair(f32x2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // V floats, as pairs where there are two.
 template <int V>
 struct Lane {
@@ -131,11 +113,6 @@ template <int V> __device__ __forceinline__ Lane<V> all_of(float v) {
 #pragma unroll
   for (int i = 0; i < (V > 1 ? V / 2 : 1); ++i) z.p[i] = pair_of(v, V > 1 ? v : 0.f);
   return z;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
 }
 template <int V> __device__ __forceinline__ float sum_of(const Lane<V> &x) {
   f32x2 s[V > 1 ? V / 2 : 1];
