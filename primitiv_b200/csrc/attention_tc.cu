@@ -8,7 +8,9 @@
 // tile's rows are in their softmax, the tensor core has the other tile's two products: per 128 keys of one tile 1024 clocks of
 // matrix instructions stand against 16384 exponentials, which are 1024 clocks of the special function units.  The products run
 // in the order in which they were issued, so p(j) v is read before s(j + 1) overwrites it.
-// 16384 causal tokens of 32 heads of 128 on 8: 1.82 ms, 1.21 PFLOP/s, at about 1.6 GHz and the GPU's 1000 W; 60 % of the tensor core's clocks.
+// 16384 causal tokens of 32 heads of 128 on 8: 1.84 ms, 1.19 PFLOP/s, in ten calls after a pause; 2.08 ms, 1.06 PFLOP/s, in a long run, where
+// the GPU's 1000 W hold the clock at about 1.55 GHz; 60 % of the tensor core's clocks.  (Figures of forms that were compared, here and below,
+// are of ten calls after a pause, on one GPU each; this form had 1.82 ms there.)
 // What is left is the way round: a softmax of 1700 clocks, two products, 600 clocks of waking one another.  Tried and no better: one place
 // for s, which the tiles have in turn, p beside it (1.83 ms); the same with pairs of blocks that share each tile of keys and
 // values, so that the tensor core reads less of shared memory (2.03 ms).
@@ -174,7 +176,7 @@ struct alignas(64) FwParams {
   int *status;
 };
 
-// Three warps on each quarter of an SM; two of the first four only lend their registers.  (16384 tokens, 32 heads of 128 on 8: 1812 us; with
+// Three warps on each quarter of an SM; two of the first four only lend their registers.  (16384 tokens, 32 heads of 128 on 8, after a pause: 1812 us; with
 // two threads a row, as the gradients have them, 2030, for what they have to tell one another; with p handed over in halves 1843.)
 constexpr uint32_t kFwThreads = 384;
 // Slots for tiles of keys and of values.
@@ -444,7 +446,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) attention_fw_tc_kernel(const __
 // Transposed where the keys rest, so that p and ds are always the left operand, from tensor memory, and a tile in shared memory
 // serves both as the right operand of the first products and of the second.  Sixteen warps share a tile: a thread has 32 of a
 // row's 128 columns.  Four warps on a scheduler fill one another's waits, and 96 registers are enough without moving any.  (6 packed sequences of up to 4096 tokens, 16 heads of 128 on 4,
-// forward and backward: 794 us with eight warps of 64 columns a thread, 753 with sixteen.)
+// forward and backward, ten calls after a pause: 794 us with eight warps of 64 columns a thread, 753 with sixteen; 868 with sixteen in a long run.)
 //   keys at rest: the sums take half of tensor memory, so s and dp have one place between them: s(i) is in registers when dp(i) is
 //     issued, and dp(i) is when s(i+1) is.  Order of the products: dp(i) s(i+1) gv(i), dp(i+1) gk(i) ...
 //     (With places of their own, p written over s and ds over dp, s(i+1) waited for gv(i) and that for p(i): 3250 clocks a step.)

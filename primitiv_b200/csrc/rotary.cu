@@ -13,7 +13,7 @@
 // forming its own, 40 heads of 128 would cost 2.6 million 64-bit products and sines per 1024 tokens instead of 65 thousand.  A
 // group stays with one token and goes over its heads, with the token's cosines and the gain in registers; arithmetic is on pairs of floats.
 // (A group that took any row, and read cosines and gain for it, spent two to three times the instructions: 71 us forward, 91 us with norms,
-// 266 us for their gradient, where this takes 62, 84 and 116; 16384 tokens of 40 heads of 128 halves.)
+// 266 us for their gradient, where this takes 61, 82 and 117; 16384 tokens of 40 heads of 128 halves.)
 // An angle is formed in turns, with what its products round off, and reduced in 64 bits, so the last position, 2^32 - 1, has the same
 // error (2^-26 of a turn) as position 1; its sine and cosine are 32-bit.
 //
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   constexpr int kUnits = kUnitsOf<V>;
   constexpr bool kSums = kNorm && kBack;
   // Where sums are kept, registers leave room for three blocks on an SM, whose loads alone do not fill the memory's latency: the next row
-  // is fetched into shared memory, where every thread has slots of its own.  (Into registers: two blocks, 199 us instead of 116.)
+  // is fetched into shared memory, where every thread has slots of its own.  (Into registers: two blocks, 199 us instead of 117.)
   constexpr bool kStaged = kSums && kUnits == 1 && V * sizeof(T) >= 8;
   constexpr uint32_t kStages = 2;   // (three or four: the same time)
   extern __shared__ float2 s_tab[];                                  // [token][V][pitch]
